@@ -26,6 +26,7 @@
 #include <vector>
 
 #include "../../include/hale_cuda.h"
+#include "hale_host.h"
 #include "hale_kernels.cuh"
 #include "hale_tc.cuh"
 #include "hale_stream.cuh"
@@ -47,57 +48,21 @@ thread_local std::string g_thread_msg;
 thread_local hale_status g_thread_status = HALE_OK;
 }  // namespace
 
-struct hale_ctx {
-    int device = 0;
-    // objects made on this context; destroying the context detaches them
-    // (their own destroy then frees their memory on their device)
-    std::set<hale_matrix*> matrices;
-    std::set<hale_pool*> pools;
-    std::set<hale_decoder*> decoders;
-    std::set<hale_comm*> comms;
-    int sm_count = 0;
-    // expert kernel family (hale_ctx_set_expert_kernel): HALE_EXPERT_AUTO =
-    // by batch shape, _TC = tcgen05 kernels, _DP4A = per-CTA kernels (dp4a /
-    // warp MMA), _PS = persistent streaming warp-MMA kernels; each where the
-    // shapes allow, else the per-CTA kernels
-    int expert_kernel = 0;
-    std::string msg;
-    hale_status status = HALE_OK;
-    uint32_t* d_err = nullptr;
-    // MoE / route workspace (capacity-based layout; counters first)
-    void* ws = nullptr;
-    size_t ws_bytes = 0;
-    int capM = 0, capE = 0, capK = 0, capH = 0, capI = 0;
-    // scratch for unit-level calls
-    void* scratch = nullptr;
-    size_t scratch_bytes = 0;
-    // bumped whenever ws or scratch is reallocated: CUDA graphs captured
-    // before hold the old addresses and must not be replayed
-    uint64_t ws_gen = 1;
-    // hale_moe_forward_host replays: one captured graph per (pool, layer,
-    // M, host buffers), valid while ws_gen matches
-    struct HostGraph {
-        const hale_pool* pool;
-        hale_moe_layer layer;
-        uint32_t M;
-        const void *x, *out, *idx, *w;
-        uint64_t gen;
-        cudaGraphExec_t exec;
-    };
-    std::vector<HostGraph> host_graphs;
-    cudaStream_t cap_st = nullptr;
-    uint32_t* h_err = nullptr;  // page-locked copy of d_err
-    uint64_t launches = 0;
-    // per-kernel event timing (hale_ctx_profile)
-    bool profiling = false;
-    struct Mark {
-        std::string name;
-        cudaEvent_t a, b;
-    };
-    std::vector<Mark> marks;
-    std::vector<cudaEvent_t> spare;
-    std::map<std::string, std::pair<uint64_t, double>> totals;
-};
+
+hale_status fail(hale_ctx* ctx, hale_status st, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_thread_msg = buf;
+    g_thread_status = st;
+    if (ctx) {
+        ctx->msg = buf;
+        ctx->status = st;
+    }
+    return st;
+}
 
 struct hale_matrix {
     hale_ctx* ctx;
@@ -148,88 +113,12 @@ struct hale_pool {
     CUtensorMap map_gu, map_d;
 };
 
-static hale_status fail(hale_ctx* ctx, hale_status st, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    g_thread_msg = buf;
-    g_thread_status = st;
-    if (ctx) {
-        ctx->msg = buf;
-        ctx->status = st;
-    }
-    return st;
-}
 
-#define CUDA_TRY(ctx, call)                                                                    \
-    do {                                                                                       \
-        cudaError_t e_ = (call);                                                               \
-        if (e_ != cudaSuccess)                                                                 \
-            return fail((ctx), e_ == cudaErrorMemoryAllocation ? HALE_E_OUT_OF_MEMORY : HALE_E_CUDA, \
-                        "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__);  \
-    } while (0)
 
-static hale_status check_launch(hale_ctx* ctx, const char* what) {
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(ctx, HALE_E_CUDA, "launch of %s failed: %s", what, cudaGetErrorString(e));
-    ctx->launches++;
-    return HALE_OK;
-}
 
-static inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
-// Opts a kernel into more than 48 KB of dynamic shared memory (once per
-// kernel and size; the attribute is per function, not per launch).
-// Static shared memory counts toward the same 48 KB default, so the opt-in
-// is made for every dynamic size, cached per device and function.
-template <class F>
-static cudaError_t allow_smem(F* func, size_t bytes) {
-    if (bytes == 0) return cudaSuccess;
-    static std::mutex mu;
-    static std::map<std::pair<int, const void*>, size_t> granted;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(mu);
-    size_t& g = granted[{dev, reinterpret_cast<const void*>(func)}];
-    if (bytes <= g) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) g = bytes;
-    return e;
-}
 
-static cudaEvent_t take_event(hale_ctx* ctx) {
-    if (!ctx->spare.empty()) {
-        cudaEvent_t e = ctx->spare.back();
-        ctx->spare.pop_back();
-        return e;
-    }
-    cudaEvent_t e = nullptr;
-    cudaEventCreate(&e);
-    return e;
-}
 
-// Brackets one launch with events when profiling is on.
-struct ProfScope {
-    hale_ctx* ctx;
-    const char* name;
-    cudaStream_t st;
-    cudaEvent_t a = nullptr;
-    ProfScope(hale_ctx* c, const char* n, cudaStream_t s) : ctx(c), name(n), st(s) {
-        if (ctx->profiling) {
-            a = take_event(ctx);
-            cudaEventRecord(a, st);
-        }
-    }
-    ~ProfScope() {
-        if (a) {
-            cudaEvent_t b = take_event(ctx);
-            cudaEventRecord(b, st);
-            ctx->marks.push_back({name, a, b});
-        }
-    }
-};
 
 static void drain_marks(hale_ctx* ctx) {
     for (auto& m : ctx->marks) {
@@ -246,19 +135,9 @@ static void drain_marks(hale_ctx* ctx) {
     cudaGetLastError();
 }
 
-static bool stream_capturing(void* stream) {
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(S(stream), &cs) != cudaSuccess) return false;
-    return cs != cudaStreamCaptureStatusNone;
-}
 
-static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-// Dynamic shared memory one CTA may ask for on sm_100 (227 KB).
-static constexpr size_t kMaxDynSmem = 227 * 1024;
 
 static bool is_quant(hale_dtype d) { return d == HALE_Q8_0 || d == HALE_Q4_0; }
-static bool is_float(hale_dtype d) { return d == HALE_F32 || d == HALE_F16 || d == HALE_BF16; }
 static int block_len(hale_dtype d) { return is_quant(d) ? 32 : 1; }
 static int block_bytes(hale_dtype d) {
     switch (d) {
@@ -270,7 +149,6 @@ static int block_bytes(hale_dtype d) {
     }
     return 0;
 }
-static int float_code(hale_dtype d) { return d == HALE_F32 ? 0 : (d == HALE_F16 ? 1 : 2); }
 
 extern "C" int64_t hale_row_bytes(hale_dtype dtype, uint64_t cols) {
     int bb = block_bytes(dtype);
@@ -336,6 +214,7 @@ extern "C" void hale_ctx_destroy(hale_ctx* ctx) {
     cudaFree(ctx->d_err);
     cudaFree(ctx->ws);
     cudaFree(ctx->scratch);
+    cudaFree(ctx->serving_ws);
     drain_marks(ctx);
     for (cudaEvent_t e : ctx->spare) cudaEventDestroy(e);
     delete ctx;

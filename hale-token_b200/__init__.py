@@ -84,6 +84,12 @@ class DecoderDesc(C.Structure):
                 ("embed", HostMatrix), ("lm_head", HostMatrix), ("final_norm", P)]
 
 
+class Kv8Struct(C.Structure):
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("table", P), ("lens", P), ("refs", P),
+                ("n_layers", U32), ("n_pages", U32), ("n_kv_heads", U32), ("head_dim", U32), ("page_tokens", U32),
+                ("n_seqs", U32), ("max_pages", U32)]
+
+
 SIGNATURES = {
     "hale_ctx_create": (I32, [C.c_int, C.POINTER(P)]),
     "hale_ctx_destroy": (None, [P]),
@@ -131,6 +137,15 @@ SIGNATURES = {
     "hale_decoder_generate": (I32, [P, P, P, U32, P, U64, U32, P, U32, P, P, P, P, P]),
     "hale_lm_head": (I32, [P, P, P, U32, P, P]),
     "hale_sample": (I32, [P, P, U32, U32, C.POINTER(SamplingParams), P, P, U32, P, P]),
+    "hale_kv8_append": (I32, [P, C.POINTER(Kv8Struct), U32, P, P, C.c_int, U64, U64, P, P, U32, P]),
+    "hale_kv8_read": (I32, [P, C.POINTER(Kv8Struct), U32, P, P, U32, P, P, C.c_int, U64, U64, P]),
+    "hale_kv8_attention": (I32, [P, C.POINTER(Kv8Struct), U32, P, C.c_int, U64, P, P, U32, U32, C.c_float, U32, U32, P,
+                                 U64, P, P]),
+    "hale_kv8_resize": (I32, [P, C.POINTER(Kv8Struct), P, P, U32, P]),
+    "hale_kv8_fork": (I32, [P, C.POINTER(Kv8Struct), P, P, U32, P]),
+    "hale_kv8_compact": (I32, [P, C.POINTER(Kv8Struct), P, P, P]),
+    "hale_kv8_copy": (I32, [P, C.POINTER(Kv8Struct), P, P, U32, P]),
+    "hale_verify_drafts": (I32, [P, P, C.c_int, U64, P, P, U64, P, U32, U32, U32, C.c_double, P, P, P, P, P]),
     "hale_expf_host": (None, [P, P, U64]),
 }
 
@@ -580,6 +595,204 @@ def sample(ctx, logits, params, rng_state, out_tokens, seen_ids=None, stream=Non
     ctx.call("hale_sample", ctx.h, ptr(logits), logits.shape[0], logits.shape[1],
              C.byref(params), ptr(rng_state), ptr(seen_ids), n_seen, ptr(out_tokens),
              _stream(stream))
+
+
+def _dtype_code(t, what):
+    import torch
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def _on(ctx, stream, **tensors):
+    """Checks that the tensors are on ctx's GPU; the stream handle to use: the
+    given one, or torch's current stream of ctx's GPU."""
+    import torch
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    if stream is None:
+        return C.c_void_p(torch.cuda.current_stream(ctx.device).cuda_stream)
+    return _stream(stream)
+
+
+def _ints(t, shape, name):
+    import torch
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+
+
+def _row_stride(t, heads, dim, name):
+    """Row stride of [n, heads, dim] with whole rows (rows may lie apart)."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
+        raise ValueError(f"{name} must be [rows, {heads}, {dim}], not {tuple(t.shape)}")
+    if t.shape[0] and ((dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim)):
+        raise ValueError(f"the values of a row of {name} must lie together")
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+class Kv8:
+    """hale_kv8: a paged key/value cache held in 8 bits.
+
+    Made over the caller's CUDA tensors (shapes in include/hale_cuda.h):
+    k, v int8 [layers, pages, kv heads, page tokens, head dim]; k_scale,
+    v_scale float32 [layers, pages, kv heads, page tokens / 16]; table int32
+    [sequences, pages a sequence can have]; lens int32 [sequences]; refs int32
+    [pages]. Kv8.empty allocates them. `seqs` and `positions` are int32 CUDA
+    tensors [rows]; seqs None is sequence 0. Refused pages, sequences and
+    positions are reported by ctx.check().
+    """
+
+    BLOCK = 16
+
+    def __init__(self, ctx, k, v, k_scale, v_scale, table, lens, refs):
+        import torch
+        if k.dim() != 5 or table.dim() != 2:
+            raise ValueError("k must be [layers, pages, kv heads, page tokens, head dim], table [sequences, pages]")
+        L, n_pages, nkv, pt, hd = k.shape
+        wants = dict(k=(k, k.shape, torch.int8), v=(v, k.shape, torch.int8),
+                     k_scale=(k_scale, (L, n_pages, nkv, pt // 16), torch.float32),
+                     v_scale=(v_scale, (L, n_pages, nkv, pt // 16), torch.float32),
+                     table=(table, table.shape, torch.int32), lens=(lens, (table.shape[0],), torch.int32),
+                     refs=(refs, (n_pages,), torch.int32))
+        for name, (t, shape, dt) in wants.items():
+            if t.dtype != dt or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dt} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+        _on(ctx, 0, k=k, v=v, k_scale=k_scale, v_scale=v_scale, table=table, lens=lens, refs=refs)
+        self.ctx = ctx
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.table, self.lens, self.refs = table, lens, refs
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page_tokens, self.head_dim = L, n_pages, nkv, pt, hd
+        self.n_seqs, self.max_pages = table.shape
+        self.c = Kv8Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+                           lens.data_ptr(), refs.data_ptr(), L, n_pages, nkv, hd, pt, self.n_seqs, self.max_pages)
+        self._ref = C.byref(self.c)
+
+    @classmethod
+    def empty(cls, ctx, n_layers, n_pages, n_kv_heads, head_dim, page_tokens, n_seqs, max_pages):
+        """A cache that holds nothing yet, on ctx's GPU."""
+        import torch
+        dev = torch.device("cuda", ctx.device)
+        codes = (n_layers, n_pages, n_kv_heads, page_tokens, head_dim)
+        scales = codes[:3] + (page_tokens // 16,)
+        return cls(ctx, torch.zeros(codes, dtype=torch.int8, device=dev), torch.zeros(codes, dtype=torch.int8, device=dev),
+                   torch.zeros(scales, device=dev), torch.zeros(scales, device=dev),
+                   torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=dev),
+                   torch.zeros(n_seqs, dtype=torch.int32, device=dev),
+                   torch.zeros(n_pages, dtype=torch.int32, device=dev))
+
+    def _rows(self, n, positions, seqs):
+        _ints(positions, (n,), "positions")
+        if seqs is not None:
+            _ints(seqs, (n,), "seqs")
+
+    def append(self, layer, k, v, positions, seqs=None, stream=None):
+        """hale_kv8_append: rows k, v [n, kv heads, head dim] become tokens
+        positions[r] of sequences seqs[r]."""
+        st = _on(self.ctx, stream, k=k, v=v, positions=positions, seqs=seqs)
+        self._rows(k.shape[0], positions, seqs)
+        if v.dtype != k.dtype or v.shape != k.shape:
+            raise ValueError("k and v must have one type and shape")
+        self.ctx.call("hale_kv8_append", self.ctx.h, self._ref, layer, ptr(k), ptr(v), _dtype_code(k, "k"),
+                      _row_stride(k, self.n_kv_heads, self.head_dim, "k"),
+                      _row_stride(v, self.n_kv_heads, self.head_dim, "v"), ptr(seqs), ptr(positions), k.shape[0], st)
+
+    def read(self, layer, k_out, v_out, positions, seqs=None, stream=None):
+        """hale_kv8_read: tokens as the values the cache stands for; either
+        output may be None."""
+        st = _on(self.ctx, stream, k_out=k_out, v_out=v_out, positions=positions, seqs=seqs)
+        some = [t for t in (k_out, v_out) if t is not None]
+        if not some:
+            return
+        if any(t.dtype != some[0].dtype for t in some):
+            raise ValueError("k_out and v_out must have one type")
+        strides = [0 if t is None else _row_stride(t, self.n_kv_heads, self.head_dim, "k_out / v_out")
+                   for t in (k_out, v_out)]
+        for t in some:
+            self._rows(t.shape[0], positions, seqs)
+        self.ctx.call("hale_kv8_read", self.ctx.h, self._ref, layer, ptr(seqs), ptr(positions), some[0].shape[0],
+                      ptr(k_out), ptr(v_out), _dtype_code(some[0], "k_out / v_out"), *strides, st)
+
+    def attention(self, layer, q, out, positions, seqs=None, scale=None, window=0, run=1, lse=None, stream=None):
+        """hale_kv8_attention: q, out [n, heads, head dim]; lse float32
+        [n, heads] or None; scale None is head_dim ** -0.5."""
+        import torch
+        st = _on(self.ctx, stream, q=q, out=out, positions=positions, seqs=seqs, lse=lse)
+        self._rows(q.shape[0], positions, seqs)
+        if out.dtype != q.dtype or out.shape != q.shape:
+            raise ValueError("q and out must have one type and shape")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+            raise ValueError(f"lse must be contiguous float32 {tuple(q.shape[:2])}")
+        self.ctx.call("hale_kv8_attention", self.ctx.h, self._ref, layer, ptr(q), _dtype_code(q, "q"),
+                      _row_stride(q, heads, self.head_dim, "q"), ptr(seqs), ptr(positions), q.shape[0], heads,
+                      self.head_dim ** -0.5 if scale is None else scale, window, run, ptr(out),
+                      _row_stride(out, heads, self.head_dim, "out"), ptr(lse), st)
+
+    def resize(self, new_lens, seqs=None, stream=None):
+        """hale_kv8_resize: sequence seqs[i] (None: i) gets length new_lens[i]."""
+        st = _on(self.ctx, stream, new_lens=new_lens, seqs=seqs)
+        self._rows(new_lens.shape[0], new_lens, seqs)
+        self.ctx.call("hale_kv8_resize", self.ctx.h, self._ref, ptr(seqs), ptr(new_lens), new_lens.shape[0], st)
+
+    def fork(self, parents, children, stream=None):
+        """hale_kv8_fork: children[i] becomes a copy of parents[i] that shares its pages."""
+        st = _on(self.ctx, stream, parents=parents, children=children)
+        _ints(parents, parents.shape[:1], "parents")
+        _ints(children, parents.shape, "children")
+        self.ctx.call("hale_kv8_fork", self.ctx.h, self._ref, ptr(parents), ptr(children), parents.shape[0], st)
+
+    def compact(self, remap, live, stream=None):
+        """hale_kv8_compact: remap int32 [2, pages], live int32 [1]."""
+        st = _on(self.ctx, stream, remap=remap, live=live)
+        _ints(remap, (2, self.n_pages), "remap")
+        _ints(live, (1,), "live")
+        self.ctx.call("hale_kv8_compact", self.ctx.h, self._ref, ptr(remap), ptr(live), st)
+
+    def copy_pages(self, src, dst, stream=None):
+        """hale_kv8_copy: pages src[i] -> dst[i] of every layer."""
+        st = _on(self.ctx, stream, src=src, dst=dst)
+        _ints(src, src.shape[:1], "src")
+        _ints(dst, src.shape, "dst")
+        self.ctx.call("hale_kv8_copy", self.ctx.h, self._ref, ptr(src), ptr(dst), src.shape[0], st)
+
+
+def verify_drafts(ctx, logits, draft_tokens, uniforms, out_tokens, out_n, draft_probs=None, n_draft=None,
+                  temperature=1.0, out_logp=None, stream=None):
+    """hale_verify_drafts: logits [batch, max_draft + 1, vocab], draft_tokens
+    int32 [batch, max_draft], uniforms float32 [batch, max_draft + 1] (None
+    when temperature <= 0), draft_probs float32 [batch, max_draft, vocab] or
+    None; out_tokens int32 [batch, max_draft + 1], out_n int32 [batch],
+    out_logp float32 like out_tokens or None."""
+    import torch
+    st = _on(ctx, stream, logits=logits, draft_tokens=draft_tokens, uniforms=uniforms, out_tokens=out_tokens,
+             out_n=out_n, draft_probs=draft_probs, n_draft=n_draft, out_logp=out_logp)
+
+    def rows(t, name):  # rows of one tensor lie a fixed stride apart
+        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1) or (
+                t.shape[0] > 1 and t.shape[1] > 0 and t.stride(0) != t.shape[1] * t.stride(1)):
+            raise ValueError(f"{name} must be [batch, rows, vocab] with rows a fixed stride apart")
+        return max(t.stride(1), t.shape[2])
+
+    stride = rows(logits, "logits")
+    B, R, V = logits.shape
+    _ints(draft_tokens, (B, R - 1), "draft_tokens")
+    _ints(out_tokens, (B, R), "out_tokens")
+    _ints(out_n, (B,), "out_n")
+    if n_draft is not None:
+        _ints(n_draft, (B,), "n_draft")
+    for name, t in (("uniforms", uniforms), ("out_logp", out_logp)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, R) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 {(B, R)}")
+    pstride = 0
+    if draft_probs is not None:
+        if draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (B, R - 1, V):
+            raise ValueError(f"draft_probs must be float32 {(B, R - 1, V)}")
+        pstride = rows(draft_probs, "draft_probs")
+    ctx.call("hale_verify_drafts", ctx.h, ptr(logits), _dtype_code(logits, "logits"), stride, ptr(draft_tokens),
+             ptr(draft_probs), pstride, ptr(n_draft), B, R - 1, V, temperature, ptr(uniforms), ptr(out_tokens),
+             ptr(out_n), ptr(out_logp), st)
 
 
 def row_bytes(dtype, cols):

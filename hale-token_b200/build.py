@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libhale_cuda.so")
-SOURCES = [os.path.join(CSRC, "hale_cuda.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("hale_cuda.cu", "hale_serving.cu")]
 DEPS = SOURCES + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))] + [
     os.path.join(ROOT, "include", "hale_cuda.h"), os.path.abspath(__file__)]
 
@@ -25,7 +25,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "--fmad=false",
     "-Xcompiler", "-fPIC,-ffp-contract=off,-fvisibility=hidden",
-    "-shared", "-cudart", "static", "-ldl",
+    "-shared", "--threads", "2", "-cudart", "static", "-ldl",
 ]
 
 

@@ -526,6 +526,132 @@ HALE_API hale_status hale_decoder_generate(hale_ctx* ctx, hale_decoder* dec, con
                                            const uint32_t* stop_tokens, uint32_t n_stop, uint32_t* out_tokens,
                                            uint32_t* n_out, float* prefill_ms, float* decode_ms, void* stream);
 
+/* ---- paged key/value cache in 8 bits ----------------------------------------
+ * Keys and values of many sequences as int8 codes, 16 consecutive tokens of a
+ * kv head sharing one f32 scale (a code c stands for c * scale): a quarter of
+ * the f32 cache's bytes. The reference keeps one growing f32 buffer per layer
+ * (src/model/attention.rs:59-85) and has no counterpart. Tokens live in pages
+ * that belong to no sequence in particular: a table names each sequence's
+ * pages, and sequences may share them.
+ *
+ * All buffers are the caller's device memory. The tables are read and written
+ * by the device, so that a captured graph replays with the lengths of the
+ * day. The calls below check what they read from them: a page number, a
+ * sequence or a position out of range is left out and reported as
+ * HALE_E_DEVICE_CHECK at the next hale_ctx_check. Calls that change the cache
+ * are ordered by their stream, like any other write to it. The first
+ * hale_kv8_attention, _resize, _compact, _copy or hale_verify_drafts call on a
+ * context allocates that context's workspace (and cannot be captured); it
+ * stays where it is until the context is destroyed. */
+#define HALE_KV8_BLOCK 16 /* tokens that share a scale */
+
+typedef struct {
+    int8_t* k;        /* [n_layers][n_pages][n_kv_heads][page_tokens][head_dim], 16-byte aligned */
+    int8_t* v;        /* same */
+    float* k_scale;   /* [n_layers][n_pages][n_kv_heads][page_tokens / 16] */
+    float* v_scale;   /* same */
+    int32_t* table;   /* [n_seqs][max_pages]: page of each page_tokens tokens; -1: none */
+    int32_t* lens;    /* [n_seqs]: tokens the sequence has room for */
+    int32_t* refs;    /* [n_pages]: table entries that name the page; 0: free */
+    uint32_t n_layers, n_pages, n_kv_heads;
+    uint32_t head_dim;    /* a multiple of 16, up to 256 */
+    uint32_t page_tokens; /* 16, 32, 64, 128 or 256 */
+    uint32_t n_seqs, max_pages;
+} hale_kv8;
+
+/* Quantises n rows of keys and values ([n_kv_heads * head_dim] floats, rows
+ * `stride` elements apart, 16-byte aligned) into layer `layer`: row r is token
+ * positions[r] of sequence seqs[r] (device arrays; seqs NULL: sequence 0). A
+ * row with a negative sequence or position is left out; of two rows for one
+ * token the later counts. The rows of one call that fall into one block of 16
+ * tokens are taken together: scale = max |x| / 127 (at least 2^-100), or the
+ * block's scale so far if that is larger; codes already in the block are
+ * rounded again when the scale grows, and a row for the block's first token
+ * starts the block anew. code = x / scale rounded half to even; NaN becomes 0
+ * and infinities the largest code, and neither sets the scale. The tokens'
+ * pages must be there (hale_kv8_resize) and be this sequence's own, which
+ * resize sees to for tokens behind the length it found. */
+HALE_API hale_status hale_kv8_append(hale_ctx* ctx, const hale_kv8* kv, uint32_t layer, const void* k, const void* v,
+                                     hale_dtype dtype, uint64_t k_stride, uint64_t v_stride, const int32_t* seqs,
+                                     const int32_t* positions, uint32_t n, void* stream);
+/* The opposite: rows as the values the cache stands for (either output may be
+ * NULL). Rows left out are not written. */
+HALE_API hale_status hale_kv8_read(hale_ctx* ctx, const hale_kv8* kv, uint32_t layer, const int32_t* seqs,
+                                   const int32_t* positions, uint32_t n, void* k_out, void* v_out, hale_dtype dtype,
+                                   uint64_t k_stride, uint64_t v_stride, void* stream);
+
+/* Attention of n query rows ([n_heads * head_dim], f32, f16 or bf16; `out`
+ * has the same type) over layer `layer`. Row r, at position p = positions[r]
+ * of sequence seqs[r] (NULL: sequence 0), sees tokens max(0, p - window + 1)
+ * .. p (window 0: all up to p); head h reads kv head h / (n_heads /
+ * n_kv_heads): out = softmax(scale * q . k) v. lse [n][n_heads] (nullable):
+ * the natural logarithm of the softmax's denominator. A row with a negative
+ * position sees nothing: out 0, lse -infinity. A row with a negative sequence
+ * is left out: nothing of it is written. `run`: how many consecutive rows of
+ * one sequence stand together at most, as far as the caller knows (1 for a
+ * decode step, the chunk's length for a prompt); results do not depend on it
+ * beyond rounding, only the kernel chosen does. Results do not change from one
+ * call to the next. */
+HALE_API hale_status hale_kv8_attention(hale_ctx* ctx, const hale_kv8* kv, uint32_t layer, const void* q,
+                                        hale_dtype dtype, uint64_t q_stride, const int32_t* seqs,
+                                        const int32_t* positions, uint32_t n, uint32_t n_heads, float scale,
+                                        uint32_t window, uint32_t run, void* out, uint64_t out_stride, float* lse,
+                                        void* stream);
+
+/* Gives sequence seqs[i] (NULL: i) the length new_lens[i] (device arrays, n up
+ * to 16384, each sequence once). Sequences that get shorter give up the pages
+ * behind their end (0 frees them all); then, in list order, those that get
+ * longer receive the free pages with the lowest numbers, and one whose last
+ * page is partly filled and shared receives its own copy of it first. All or
+ * nothing: with too few free pages, or a bad argument, nothing changes and
+ * hale_ctx_check reports HALE_E_DEVICE_CHECK. */
+HALE_API hale_status hale_kv8_resize(hale_ctx* ctx, const hale_kv8* kv, const int32_t* seqs, const int32_t* new_lens,
+                                     uint32_t n, void* stream);
+/* Sequence children[i] gives up what it holds and becomes a copy of
+ * parents[i] that shares all its pages. Each child once, and no child a
+ * parent in the same call (else nothing changes and HALE_E_DEVICE_CHECK). */
+HALE_API hale_status hale_kv8_fork(hale_ctx* ctx, const hale_kv8* kv, const int32_t* parents, const int32_t* children,
+                                   uint32_t n, void* stream);
+/* Moves the pages in use to the front: with L of them, pages 0 .. L-1 hold
+ * everything afterwards and the tables are renumbered. remap [2][n_pages]: the
+ * new number of every page (-1: was free), then the old number of every page
+ * (-1: free now). live [1]: L. Pages at or above L keep stale bytes. */
+HALE_API hale_status hale_kv8_compact(hale_ctx* ctx, const hale_kv8* kv, int32_t* remap, int32_t* live, void* stream);
+/* Copies pages src[i] -> dst[i] (device arrays) in every layer, codes and
+ * scales; tables and counts stay. Each dst once, and no dst a src too, except
+ * of itself (else nothing is copied and HALE_E_DEVICE_CHECK). */
+HALE_API hale_status hale_kv8_copy(hale_ctx* ctx, const hale_kv8* kv, const int32_t* src, const int32_t* dst, uint32_t n,
+                                   void* stream);
+
+/* ---- drafted tokens ----------------------------------------------------------
+ * Speculative sampling's check, the counterpart of Sampler::sample
+ * (src/generate/sampler.rs:80-123) for several drafted tokens at once; the
+ * reference has none. Sequence b drafted n = n_draft[b] tokens (NULL:
+ * max_draft; up to 64) draft_tokens[b][0 .. n-1]; logits holds max_draft + 1
+ * rows of the target per sequence (f32, f16 or bf16, rows logits_stride
+ * elements apart), row i for the place of drafted token i. With p_i =
+ * softmax(logits_i / temperature) and the draft's probabilities q_i
+ * (draft_probs [batch][max_draft] rows of f32, probs_stride apart; NULL: the
+ * draft was certain of its token), token i is kept while u_i q_i(x_i) <
+ * p_i(x_i), u = uniforms[b][0 .. max_draft]; the first that is not is replaced
+ * by a draw from max(p_i - q_i, 0), and when all are kept a draw from p_n
+ * follows. A draw takes the lowest token whose cumulated probability exceeds
+ * uniforms[b][max_draft] times the whole. temperature <= 0: a token is kept
+ * while it is the row's largest logit (the lowest of equals), which also takes
+ * the place of the draw. A top-k or nucleus cut is the caller's, as -infinity
+ * in the logits; NaN counts as -infinity. out_tokens [batch][max_draft + 1]:
+ * the kept tokens, the drawn one, then -1; out_n [batch]: how many; out_logp
+ * (nullable, same shape): log p of each (temperature <= 0: of the softmax of
+ * the logits), 0 behind them. A row with nothing above -infinity keeps nothing
+ * and draws nothing. A drafted token outside the vocabulary, or a count
+ * outside 0 .. max_draft, is not kept and reported as HALE_E_DEVICE_CHECK.
+ * batch * (max_draft + 1) up to 65535, vocab up to 2^24. */
+HALE_API hale_status hale_verify_drafts(hale_ctx* ctx, const void* logits, hale_dtype dtype, uint64_t logits_stride,
+                                        const int32_t* draft_tokens, const float* draft_probs, uint64_t probs_stride,
+                                        const int32_t* n_draft, uint32_t batch, uint32_t max_draft, uint32_t vocab,
+                                        double temperature, const float* uniforms, int32_t* out_tokens, int32_t* out_n,
+                                        float* out_logp, void* stream);
+
 /* ---- self-checks ----------------------------------------------------------- */
 
 /* The exp used by the device kernels, evaluated on the host from the same

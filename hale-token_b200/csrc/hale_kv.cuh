@@ -626,87 +626,4 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvArgs c, int n_layers, co
     }
 }
 
-// ---------------------------------------------------------------------------
-// attention
-//
-// Row r of a sequence at position p, query head h over kv head h / (nh / nkv):
-//   s_t = scale * sum_d q_d k_td,  t = max(0, p - window + 1) .. p
-//   out = sum_t softmax(s)_t v_t,  lse = log sum_t exp(s_t)
-// ---------------------------------------------------------------------------
-struct KvAttn {
-    const void* q;
-    void* out;
-    float* lse;
-    const int32_t *seqs, *positions;
-    size_t q_stride, out_stride;
-    int n, nh, group, window;
-    float scale;
-};
-
-// One CTA per (row, query head), four warps on alternating tokens, lanes over
-// the head's dims; each warp keeps the running maximum, sum and weighted sum
-// of a softmax in f32, joined at the end.
-template <int DT>
-__global__ void __launch_bounds__(128) kv_attention_kernel(KvArgs c, KvAttn a) {
-    __shared__ float s_m[4], s_l[4], s_o[4][256];
-    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int seq = a.seqs ? a.seqs[row] : 0, head = h / a.group;
-    if (seq < 0) return;
-    int end = a.positions[row] + 1;
-    if (seq >= c.n_seqs || end > c.capacity()) {
-        if (threadIdx.x == 0) raise_error(c.err, kErrBounds);
-        end = 0;
-    }
-    const int begin = a.window > 0 ? max(0, end - a.window) : 0;
-    float q[8], o[8], m = -__int_as_float(0x7f800000), l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int d = lane + 32 * i;
-        q[i] = d < c.hd ? load1<DT>(a.q, (size_t)row * a.q_stride + (size_t)h * c.hd + d) : 0.0f;
-        o[i] = 0.0f;
-    }
-    for (int t = begin + warp; t < end; t += 4) {
-        const int page = c.page_of(c.table, seq, t), slot = c.slot(t);
-        if (page < 0) {
-            raise_error(c.err, kErrBounds);
-            continue;
-        }
-        const size_t at = c.code_at(page, head, slot), sa = c.scale_at(page, head, slot);
-        float s = 0.0f, v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = lane + 32 * i;
-            const bool in = d < c.hd;
-            s = fmaf(q[i], in ? (float)c.k[at + d] : 0.0f, s);
-            v[i] = in ? (float)c.v[at + d] : 0.0f;
-        }
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= c.ks[sa] * a.scale;
-        const float top = fmaxf(m, s), fix = expf(m - top), p = expf(s - top), f = p * c.vs[sa];
-        l = l * fix + p;
-        m = top;
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = fmaf(f, v[i], o[i] * fix);
-    }
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-#pragma unroll
-    for (int i = 0; i < 8; i++) s_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), sum = 0.0f, f[4];
-    const bool empty = !(top > -__int_as_float(0x7f800000)) && top == top;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        f[w] = empty || s_l[w] == 0.0f ? 0.0f : expf(s_m[w] - top);
-        sum += f[w] * s_l[w];
-    }
-    for (int d = threadIdx.x; d < c.hd; d += 128) {
-        float x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) x += f[w] * s_o[w][d];
-        store1<DT>(a.out, (size_t)row * a.out_stride + (size_t)h * c.hd + d, empty ? 0.0f : x / sum);
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[(size_t)row * a.nh + h] = empty ? -__int_as_float(0x7f800000) : top + logf(sum);
-}
-
 }  // namespace hale

@@ -4,6 +4,7 @@
 #include "hale_host.h"
 
 #include "hale_kv.cuh"
+#include "hale_kv_attn.cuh"
 #include "hale_verify.cuh"
 
 #include <algorithm>
@@ -36,13 +37,17 @@ struct ServingWs {
     static constexpr size_t kPairsOff = 256;
     static constexpr size_t kPairsBytes = (size_t)kMaxKvPages / 2 * 4;
     static constexpr size_t kPartsOff = kPairsOff + 2 * kPairsBytes;
-    static constexpr size_t kTotal = kPartsOff + (size_t)kVerifyParts * sizeof(VerifyPart);
+    static constexpr size_t kArrivedOff = kPartsOff + (size_t)kVerifyParts * sizeof(VerifyPart);
+    static constexpr size_t kAttnOff = kArrivedOff + kAttnMaxGrid * 4;
+    static constexpr size_t kTotal = kAttnOff + kAttnPartBytes;
     uint8_t* base;
     PagePairs pairs() const {
         return {reinterpret_cast<int32_t*>(base), reinterpret_cast<int32_t*>(base + kPairsOff),
                 reinterpret_cast<int32_t*>(base + kPairsOff + kPairsBytes)};
     }
     VerifyPart* parts() const { return reinterpret_cast<VerifyPart*>(base + kPartsOff); }
+    unsigned* arrived() const { return reinterpret_cast<unsigned*>(base + kArrivedOff); }
+    float* attn_parts() const { return reinterpret_cast<float*>(base + kAttnOff); }
 };
 
 hale_status serving_ws(hale_ctx* ctx, void* stream, ServingWs* out) {
@@ -130,6 +135,44 @@ hale_status check_layer_rows(hale_ctx* ctx, const hale_kv8* kv, const char* what
     if (n > kMaxRows) return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: %u rows (up to 2^22)", what, n);
     if (!positions) return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: positions is NULL", what);
     return HALE_OK;
+}
+
+// CTAs of an attention launch: what the GPU holds at once, no more than there
+// can be units of CH tokens, and no more than the workspace has parts for.
+unsigned attn_grid(const hale_ctx* ctx, const KvArgs& c, const KvAttn& a, int per_sm, int chunk) {
+    const uint64_t units = (uint64_t)a.n * c.nkv * a.subs * (((uint64_t)c.capacity() + chunk - 1) / chunk);
+    const uint64_t parts = kAttnPartBytes / 8 / a.part_floats;
+    return (unsigned)std::min<uint64_t>({(uint64_t)ctx->sm_count * per_sm, units, parts, (uint64_t)kAttnMaxGrid});
+}
+
+template <int DT, int DP, int NT>
+hale_status attn_few(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cudaStream_t st) {
+    constexpr int cols = 8 * NT;
+    a.heads = std::min(a.group, cols);
+    a.subs = (a.group + a.heads - 1) / a.heads;
+    a.rows = (int)std::max<uint32_t>(1u, std::min<uint32_t>(run, (uint32_t)(cols / a.heads)));
+    a.part_floats = cols * (2 + c.hd);
+    const size_t smem = (size_t)kFewWarps * cols * DP * 4;
+    CUDA_TRY(ctx, allow_smem(kv_attn_few_kernel<DT, DP, NT>, smem));
+    const unsigned grid = attn_grid(ctx, c, a, DP <= 128 && NT == 1 ? 3 : 2, FewCfg<DP>::CH);
+    kv_attn_few_kernel<DT, DP, NT><<<grid, kFewThreads, smem, st>>>(c, a);
+    return check_launch(ctx, "kv_attn_few");
+}
+
+template <int DT, int NT>
+hale_status attn_few_dim(hale_ctx* ctx, const KvArgs& c, const KvAttn& a, uint32_t run, cudaStream_t st) {
+    if (c.hd <= 64) return attn_few<DT, 64, NT>(ctx, c, a, run, st);
+    if (c.hd <= 128) return attn_few<DT, 128, NT>(ctx, c, a, run, st);
+    return attn_few<DT, 256, NT>(ctx, c, a, run, st);
+}
+
+template <int DT>
+hale_status attn_go(hale_ctx* ctx, const KvArgs& c, const KvAttn& a, uint32_t run, cudaStream_t st) {
+    const uint64_t cols = (uint64_t)std::min<uint32_t>(run, (uint32_t)a.n) * a.group;
+    if (cols <= 8) return attn_few_dim<DT, 1>(ctx, c, a, run, st);
+    if (cols <= 16) return attn_few_dim<DT, 2>(ctx, c, a, run, st);
+    kv_attention_kernel<DT><<<dim3(a.n, a.nh), 128, 0, st>>>(c, a);
+    return check_launch(ctx, "kv_attention");
 }
 
 template <int DT>
@@ -235,14 +278,16 @@ extern "C" hale_status hale_kv8_attention(hale_ctx* ctx, const hale_kv8* kv, uin
     a.group = (int)(n_heads / kv->n_kv_heads);
     a.window = (int)std::min<uint32_t>(window, 0x7fffffffu);
     a.scale = scale;
+    ServingWs ws;
+    if ((r = serving_ws(ctx, stream, &ws))) return r;
+    a.parts = ws.attn_parts();
+    a.arrived = ws.arrived();
     ProfScope ps(ctx, "kv8_attention", S(stream));
-    const dim3 grid(n, n_heads);
     switch (dtype) {
-    case HALE_F32: kv_attention_kernel<0><<<grid, 128, 0, S(stream)>>>(c, a); break;
-    case HALE_F16: kv_attention_kernel<1><<<grid, 128, 0, S(stream)>>>(c, a); break;
-    default: kv_attention_kernel<2><<<grid, 128, 0, S(stream)>>>(c, a); break;
+    case HALE_F32: return attn_go<0>(ctx, c, a, run, S(stream));
+    case HALE_F16: return attn_go<1>(ctx, c, a, run, S(stream));
+    default: return attn_go<2>(ctx, c, a, run, S(stream));
     }
-    return check_launch(ctx, "kv_attention");
 } catch (...) {
     return HALE_E_OUT_OF_MEMORY;
 }

@@ -5,11 +5,11 @@
 //   out = sum_t softmax(s)_t vs_b(t) vc_t,     lse = log sum_t exp(s_t)
 // with int8 codes kc, vc and one scale per block b of 16 tokens. The scales
 // multiply whole scores and whole softmax weights, so the products run on the
-// codes themselves: an int8 is exact in f16, and both products are f16 matrix
-// products with 32-bit sums.
-//   - q is scaled by a power of two to at most 2^14 and rounded to f16: exact
-//     for f16 and (down to 2^-31 of the row's largest value) for bf16; f32 is
-//     held as two f16 (22 bits).
+// codes themselves.
+//   - q is scaled by a power of two and rounded to an integer below 2^23, held
+//     as three int8 digits in base 256 (off by at most 2^-23 of the row's
+//     largest value, an f32's own last place there): q . kc is three int8
+//     matrix products, exact in 32-bit integers.
 //   - a softmax weight times its block's value scale, over the largest such
 //     scale so far and times 2^14, is rounded to f16 (11 bits, the accuracy of
 //     the result's own type or better); for f32 results to two f16 (22 bits).
@@ -285,13 +285,35 @@ __device__ __forceinline__ uint2 load_stream8(const void* p) {
 constexpr float kWeightTop = 16384.0f;  // the largest weight as f16
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// Power of two that brings amax to at most 2^14 and at least 2^13 (1 for 0 and
-// for values that are not finite).
+// Power of two that brings amax below 2^22.99 and to at least 2^21.99 (1 for 0
+// and for values that are not finite).
 __device__ __forceinline__ float kv_query_scale(float amax) {
     if (!(amax > 0.0f) || !(amax <= 0x1.fffffep127f)) return 1.0f;
     int e;
-    frexpf(amax, &e);  // amax < 2^e
-    return ldexpf(1.0f, min(126, max(-126, 14 - e)));
+    const float f = frexpf(amax, &e);  // amax = f 2^e, f in [1/2, 1)
+    // the digits reach 127 * 65793 < 2^23: f must stay below 0.996
+    return ldexpf(1.0f, min(126, max(-126, (f < 0.99f ? 23 : 22) - e)));
+}
+
+// Four values as one register of each of the three digits of their integers:
+// x = d0 65536 + d1 256 + d2, d1 and d2 in [-128, 127].
+__device__ __forceinline__ void kv_query_digits(const float (&x)[4], uint32_t (&d)[3]) {
+    d[0] = d[1] = d[2] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int n = __float2int_rn(x[i]);
+        const int lo = (int8_t)n, n1 = (n - lo) >> 8, mid = (int8_t)n1, hi = (n1 - mid) >> 8;
+        d[0] |= (uint32_t)(hi & 0xff) << (8 * i);
+        d[1] |= (uint32_t)(mid & 0xff) << (8 * i);
+        d[2] |= (uint32_t)(lo & 0xff) << (8 * i);
+    }
+}
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // ---------------------------------------------------------------------------
@@ -299,14 +321,16 @@ __device__ __forceinline__ float kv_query_scale(float amax) {
 //
 // Four warps, each on its own 16 NB tokens of a unit. Keys: a lane loads 16
 // consecutive dims of two tokens, which are (after a permutation of the dims
-// that the query's fragment repeats) four A fragments of 16 tokens x 16 dims:
-// no shared memory between HBM and the tensor core. S^T = K q^T leaves a
-// column's scores in the lanes of one quad position, so its weights, moved
-// through one 8x8 transpose, are the B fragment of O^T = V^T P^T; V's A
-// fragments are again bytes of a lane's own loads (four tokens, 2 DP/16
-// consecutive dims), paired by byte permutes.
-// Bound by reading the codes.
-// ---------------------------------------------------------------------------
+// that the query's fragment repeats) A fragments of 16 tokens x 32 dims as they
+// stand: nothing between HBM and the tensor core. S^T = K q^T leaves a column's
+// scores in the lanes of one quad position, so its weights, moved through an
+// 8x8 transpose, are the B fragment of O^T = V^T P^T, an f16 product (weights
+// span many orders of magnitude, which integers would cut off); V's A fragments
+// are again bytes of a lane's own loads (four tokens, DP / 8 consecutive dims),
+// paired by byte permutes and widened to f16.
+// Every load is made, hidden tokens and dims past the head's included (at an
+// address that is there): codes are finite whatever they are, and a hidden
+// token's weight, like a missing dim of q, is 0.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 
 template <int DP>
@@ -317,7 +341,8 @@ struct FewCfg {
     static constexpr int VW = DP / 32;                   // 32-bit words of a lane's dims of one value row
 };
 
-template <int DT, int DP, int NT>
+// HD: the head's dims where they are known (= DP), else 0.
+template <int DT, int DP, int HD, int NT>
 __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_attn_few_kernel(KvArgs c, KvAttn a) {
     using Cfg = FewCfg<DP>;
     constexpr int NB = Cfg::NB, CH = Cfg::CH, KC = Cfg::KC, VW = Cfg::VW, MT = DP / 16, COLS = 8 * NT;
@@ -328,6 +353,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
     __shared__ int s_last;
     extern __shared__ __align__(16) float s_acc[];  // [kFewWarps][COLS][DP]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+    const int hd = HD ? HD : c.hd;
     const float none = -__int_as_float(0x7f800000);
 
     KvWalk<CH, kFewThreads> walk;
@@ -343,7 +369,9 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         const int h0 = head * a.group + sub * a.heads;  // the tile's first query head
 
         // ---- the columns' queries, as B fragments, and what they see ----
-        uint32_t qf[SPLIT][NT][KC * 4][2];
+        // (the integer product's k index runs over 16 t + 4 q4 + byte of a
+        // 32-dim step: words 0, 1 and 2, 3 of a lane's 16 dims)
+        uint32_t qf[3][NT][KC * 2][2];
         float qs[NT][2];
         int end[NT][2], begin[NT][2];
         int all_lo = 0, all_hi = INT_MAX;  // tokens every column sees
@@ -351,42 +379,43 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         for (int nt = 0; nt < NT; nt++) {
             const int col = nt * 8 + g;
             const bool in = col < cols;
-            const size_t at = in ? (size_t)(seg.row + col / heads) * a.q_stride + (size_t)(h0 + col % heads) * c.hd : 0;
-            float x[KC][16];
+            const size_t at = in ? (size_t)(seg.row + col / heads) * a.q_stride + (size_t)(h0 + col % heads) * hd : 0;
+            float x[KC][4][4];
             float amax = 0.0f;
 #pragma unroll
             for (int p = 0; p < KC; p++) {
                 const int d = 64 * p + 16 * q4;
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (in && d < c.hd) load4<DT>(a.q, at + d + e, y);
+                for (int w = 0; w < 4; w++) {
+                    x[p][w][0] = x[p][w][1] = x[p][w][2] = x[p][w][3] = 0.0f;
+                    if (in && d < hd) load4<DT>(a.q, at + d + 4 * w, x[p][w]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        x[p][e + i] = y[i];
-                        amax = fmaxf(amax, fabsf(y[i]));
-                    }
+                    for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(x[p][w][i]));
                 }
             }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const float up = kv_query_scale(amax);
+            bool wild = false;  // infinities and NaN have no digits
 #pragma unroll
             for (int p = 0; p < KC; p++)
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    float y[4];
+                for (int w = 0; w < 4; w++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) y[i] = x[p][4 * t + i] * up;
-                    qf[0][nt][4 * p + t][0] = pack_f16(y[0], y[2]);
-                    qf[0][nt][4 * p + t][1] = pack_f16(y[1], y[3]);
-                    if (SPLIT == 2) {
+                    for (int i = 0; i < 4; i++) wild |= !(fabsf(x[p][w][i]) <= 0x1.fffffep127f);
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const unsigned wilds = __ballot_sync(0xffffffffu, wild);
+            float up = kv_query_scale(amax);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) y[i] -= __half2float(__float2half_rn(y[i]));
-                        qf[SPLIT - 1][nt][4 * p + t][0] = pack_f16(y[0], y[2]);
-                        qf[SPLIT - 1][nt][4 * p + t][1] = pack_f16(y[1], y[3]);
-                    }
+            for (int p = 0; p < KC; p++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t d[3];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[p][w][i] *= up;
+                    kv_query_digits(x[p][w], d);
+#pragma unroll
+                    for (int z = 0; z < 3; z++) qf[z][nt][2 * p + (w >> 1)][w & 1] = d[z];
                 }
+            if (wilds >> (4 * g) & 15u) up = __int_as_float(0x7fc00000);  // the column's scores become NaN
             // the scores' columns are 2 q4 and 2 q4 + 1 of the lane
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -415,22 +444,27 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
             for (int i = 0; i < MT; i++) acc[i][nt][0] = acc[i][nt][1] = acc[i][nt][2] = acc[i][nt][3] = 0.0f;
         }
         const int32_t* row = c.table + (size_t)min(seg.seq, c.n_seqs - 1) * c.max_pages;
+        // a page's codes and scales (at most 2^26 bytes), and this lane's place in a block
+        const unsigned page_codes = (unsigned)(c.nkv * hd) << c.page_log2, page_scales = (unsigned)c.nkv << c.page_log2 >> 4;
+        const int8_t* kbase = c.k + ((size_t)head << c.page_log2) * hd + (unsigned)(g * hd) + (HD ? 16 * q4 : 0);
+        const int8_t* vbase = c.v + ((size_t)head << c.page_log2) * hd + (unsigned)(2 * q4 * hd) + (HD ? 4 * VW * g : 0);
+        const float* ksbase = c.ks + ((size_t)head << c.page_log2 >> 4);
+        const float* vsbase = c.vs + ((size_t)head << c.page_log2 >> 4);
 
         // ---- tokens ----
         uint4 kr[NB][2][KC];          // tokens g and g + 8 of each block
         uint32_t vr[NB][4][VW];       // tokens 2 q4, + 1, + 8, + 9
         float ks[NB], vs[NB], ks_next[NB], vs_next[NB];
         int page[NB], page_next[NB];
-        // page of each block of unit u: -1 nothing to see there, -2 missing
+        // page of each block of unit u, -1: nothing of it is seen, or it is missing
         auto find = [&](int u, int (&pg)[NB]) {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const int t = u * CH + warp * Cfg::TB + 16 * b;
                 pg[b] = -1;
                 if (u < u1 && t < seg.hi && t + 16 > seg.lo) {
-                    const int p = c.checked(row[t >> c.page_log2]);
-                    if (p < 0 && lane == 0) raise_error(c.err, kErrBounds);
-                    pg[b] = p;
+                    pg[b] = c.checked(row[t >> c.page_log2]);
+                    if (pg[b] < 0 && lane == 0) raise_error(c.err, kErrBounds);
                 }
             }
         };
@@ -438,39 +472,35 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * b);
-                fk[b] = fv[b] = 0.0f;
+                const unsigned pn = (unsigned)max(pg[b], 0);
+                fk[b] = ksbase[(size_t)pn * page_scales + (slot >> 4)];
+                fv[b] = vsbase[(size_t)pn * page_scales + (slot >> 4)];
+                if (pg[b] < 0) fk[b] = fv[b] = 0.0f;
+                const int8_t* src = kbase + (size_t)pn * page_codes + (unsigned)(slot * hd);
 #pragma unroll
-                for (int p = 0; p < KC; p++) kr[b][0][p] = kr[b][1][p] = make_uint4(0, 0, 0, 0);
-                if (pg[b] < 0) continue;
-                const size_t sa = c.scale_at(pg[b], head, slot);
-                fk[b] = c.ks[sa];
-                fv[b] = c.vs[sa];
-                const int8_t* src = c.k + c.code_at(pg[b], head, slot) + 16 * q4;
-#pragma unroll
-                for (int p = 0; p < KC; p++)
-                    if (64 * p + 16 * q4 < c.hd) {
-                        kr[b][0][p] = load_stream16(src + (size_t)g * c.hd + 64 * p);
-                        kr[b][1][p] = load_stream16(src + (size_t)(g + 8) * c.hd + 64 * p);
-                    }
+                for (int p = 0; p < KC; p++) {
+                    const int d = HD ? 64 * p : min(64 * p + 16 * q4, hd - 16);
+                    kr[b][0][p] = load_stream16(src + d);
+                    kr[b][1][p] = load_stream16(src + 8 * hd + d);
+                }
             }
         };
         auto load_v = [&](int u, const int (&pg)[NB]) {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * b);
-                const int8_t* src = c.v + c.code_at(max(pg[b], 0), head, slot) + 4 * VW * g;
+                const int8_t* src = vbase + (size_t)(unsigned)max(pg[b], 0) * page_codes + (unsigned)(slot * hd);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int8_t* p = src + (size_t)(2 * q4 + (j & 1) + 8 * (j >> 1)) * c.hd;
+                    const int8_t* p = src + ((j & 1) + 8 * (j >> 1)) * hd;
                     if (VW == 2) {
-                        const uint2 v = pg[b] >= 0 && 8 * g < c.hd ? load_stream8(p) : make_uint2(0, 0);
+                        const uint2 v = load_stream8(p);
                         vr[b][j][0] = v.x;
                         vr[b][j][1] = v.y;
                     } else {
 #pragma unroll
                         for (int w = 0; w + 4 <= VW; w += 4) {
-                            const uint4 v = pg[b] >= 0 && 4 * VW * g + 4 * w < c.hd ? load_stream16(p + 4 * w)
-                                                                                    : make_uint4(0, 0, 0, 0);
+                            const uint4 v = load_stream16(p + (HD ? 4 * w : min(4 * VW * g + 4 * w, hd - 16)));
                             vr[b][j][w] = v.x;
                             vr[b][j][w + 1] = v.y;
                             vr[b][j][w + 2] = v.z;
@@ -486,47 +516,71 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         find(u0 + 1, page_next);
         for (int u = u0; u < u1; u++) {
             const int t0 = u * CH + warp * Cfg::TB;
-            float s[NB][NT][4];
+            const bool more = u + 1 < u1;
+            float s[NB][NT][4];  // q . kc as integers of at most 2^45, rounded to f32
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[b][nt][0] = s[b][nt][1] = s[b][nt][2] = s[b][nt][3] = 0.0f;
+                for (int nt = 0; nt < NT; nt++) {
+                    int z0[4] = {0, 0, 0, 0}, z1[4] = {0, 0, 0, 0}, z2[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int p = 0; p < KC; p++) {
-                    const uint32_t x[4] = {kr[b][0][p].x, kr[b][0][p].y, kr[b][0][p].z, kr[b][0][p].w};
-                    const uint32_t y[4] = {kr[b][1][p].x, kr[b][1][p].y, kr[b][1][p].z, kr[b][1][p].w};
-#pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        const uint32_t a0 = codes_even(x[t]), a1 = codes_even(y[t]), a2 = codes_odd(x[t]), a3 = codes_odd(y[t]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int z = 0; z < SPLIT; z++)
-                                mma_f16(s[b][nt], a0, a1, a2, a3, qf[z][nt][4 * p + t][0], qf[z][nt][4 * p + t][1]);
+                    for (int p = 0; p < KC; p++) {
+                        const uint4 x = kr[b][0][p], y = kr[b][1][p];
+                        mma_s8(z0, x.x, y.x, x.y, y.y, qf[0][nt][2 * p][0], qf[0][nt][2 * p][1]);
+                        mma_s8(z1, x.x, y.x, x.y, y.y, qf[1][nt][2 * p][0], qf[1][nt][2 * p][1]);
+                        mma_s8(z2, x.x, y.x, x.y, y.y, qf[2][nt][2 * p][0], qf[2][nt][2 * p][1]);
+                        mma_s8(z0, x.z, y.z, x.w, y.w, qf[0][nt][2 * p + 1][0], qf[0][nt][2 * p + 1][1]);
+                        mma_s8(z1, x.z, y.z, x.w, y.w, qf[1][nt][2 * p + 1][0], qf[1][nt][2 * p + 1][1]);
+                        mma_s8(z2, x.z, y.z, x.w, y.w, qf[2][nt][2 * p + 1][0], qf[2][nt][2 * p + 1][1]);
                     }
-                }
-            load_k(u + 1, page_next, ks_next, vs_next);
-            // scores in units of log 2, hidden tokens -inf
-            bool whole = t0 >= all_lo && t0 + Cfg::TB <= all_hi;
 #pragma unroll
-            for (int b = 0; b < NB; b++) whole = whole && page[b] >= 0;
-            bool raise = false;
+                    for (int e = 0; e < 4; e++)  // |z| <= 2^22: z1 256 + z2 fits 32 bits
+                        s[b][nt][e] = fmaf((float)z0[e], 65536.0f, (float)(z1[e] * 256 + z2[e]));
+                }
+            if (more) load_k(u + 1, page_next, ks_next, vs_next);
+            // score = s f in units of log 2
+            float f[NB][NT][2];
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = s[b][nt][e] * (ks[b] * qs[nt][e & 1]);
-                        if (!whole) {
+                    for (int e = 0; e < 2; e++) f[b][nt][e] = ks[b] * qs[nt][e];
+            bool whole = t0 >= all_lo && t0 + Cfg::TB <= all_hi;
+#pragma unroll
+            for (int b = 0; b < NB; b++) whole = whole && page[b] >= 0;
+            unsigned hidden = 0;  // bit (b NT + nt) 4 + e
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
                             const int t = t0 + 16 * b + g + 8 * (e >> 1);
-                            if (page[b] < 0 || t >= end[nt][e & 1] || t < begin[nt][e & 1]) x = none;
+                            if (page[b] < 0 || t >= end[nt][e & 1] || t < begin[nt][e & 1])
+                                hidden |= 1u << ((b * NT + nt) * 4 + e);
                         }
-                        s[b][nt][e] = x;
-                        raise |= x > m[nt][e & 1];
+            }
+            float top[NT][2];
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float x = m[nt][e];
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        float y0 = s[b][nt][e] * f[b][nt][e], y1 = s[b][nt][e + 2] * f[b][nt][e];
+                        if (!whole) {
+                            y0 = hidden >> ((b * NT + nt) * 4 + e) & 1u ? none : y0;
+                            y1 = hidden >> ((b * NT + nt) * 4 + e + 2) & 1u ? none : y1;
+                        }
+                        x = fmaxf(x, fmaxf(y0, y1));
                     }
+                    top[nt][e] = x;
+                    raise |= x > m[nt][e];
+                }
             float vmax = vtop;
 #pragma unroll
             for (int b = 0; b < NB; b++) vmax = fmaxf(vmax, vs[b]);
@@ -538,19 +592,17 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float top = m[nt][e];
-#pragma unroll
-                        for (int b = 0; b < NB; b++) top = fmaxf(top, fmaxf(s[b][nt][e], s[b][nt][e + 2]));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float fix = m[nt][e] == none ? 0.0f : exp2_fast(m[nt][e] - top);
-                        m[nt][e] = top;
+                        float x = top[nt][e];
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float fix = m[nt][e] == none ? 0.0f : exp2_fast(m[nt][e] - x), fix_acc = fix * fix_v;
+                        m[nt][e] = x;
                         l[nt][e] *= fix;
 #pragma unroll
                         for (int i = 0; i < MT; i++) {
-                            acc[i][nt][e] *= fix * fix_v;
-                            acc[i][nt][e + 2] *= fix * fix_v;
+                            acc[i][nt][e] *= fix_acc;
+                            acc[i][nt][e + 2] *= fix_acc;
                         }
                     }
             }
@@ -564,8 +616,10 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float top = m[nt][e & 1];
-                        const float p = exp2_fast(s[b][nt][e] - (top == none ? 0.0f : top));
+                        // one rounding between the product and its distance from the maximum
+                        const float base = m[nt][e & 1] == none ? 0.0f : m[nt][e & 1];
+                        float p = exp2_fast(fmaf(s[b][nt][e], f[b][nt][e & 1], -base));
+                        if (!whole) p = hidden >> ((b * NT + nt) * 4 + e) & 1u ? 0.0f : p;
                         l[nt][e & 1] += p;
                         w[e] = p * fv;
                     }
@@ -593,14 +647,16 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                         }
                 }
             }
-            load_v(u + 1, page_next);
+            if (more) {
+                load_v(u + 1, page_next);
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                page[b] = page_next[b];
-                ks[b] = ks_next[b];
-                vs[b] = vs_next[b];
+                for (int b = 0; b < NB; b++) {
+                    page[b] = page_next[b];
+                    ks[b] = ks_next[b];
+                    vs[b] = vs_next[b];
+                }
+                find(u + 2, page_next);
             }
-            find(u + 2, page_next);
         }
 
         // ---- the four warps' parts joined ----
@@ -645,7 +701,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         }
         __syncthreads();
         const bool split = tile0 < walk.begin || tile1 > walk.end;
-        const int quads = c.hd / 4;
+        const int quads = hd / 4;
         int c0 = 0, c1 = 0;
         if (split) {
             // this CTA's part to the workspace; the last to arrive joins them
@@ -660,7 +716,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                     const float4 y = *reinterpret_cast<const float4*>(s_acc + ((size_t)w * COLS + k) * DP + d);
                     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
                 }
-                __stcg(reinterpret_cast<float4*>(part + 2 * COLS + (size_t)k * c.hd + d), x);
+                __stcg(reinterpret_cast<float4*>(part + 2 * COLS + (size_t)k * hd + d), x);
             }
             if (tid < cols) {
                 __stcg(part + tid, s_f[tid]);
@@ -696,7 +752,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                     for (int r = c0; r <= c1; r++) {
                         const float* part = a.parts + ((size_t)2 * r + (r == c0)) * a.part_floats;
                         const float mr = __ldcg(part + k), f = mr == none ? 1.0f : exp2_fast(mr - top);
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part + 2 * COLS + (size_t)k * c.hd + d));
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part + 2 * COLS + (size_t)k * hd + d));
                         sum += f * __ldcg(part + COLS + k);
                         x[0] = fmaf(f, y.x, x[0]); x[1] = fmaf(f, y.y, x[1]);
                         x[2] = fmaf(f, y.z, x[2]); x[3] = fmaf(f, y.w, x[3]);
@@ -707,7 +763,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 const float inv = empty ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[e] = empty ? 0.0f : x[e] * inv;
-                store4<DT>(a.out, (size_t)r * a.out_stride + (size_t)h * c.hd + d, x);
+                store4<DT>(a.out, (size_t)r * a.out_stride + (size_t)h * hd + d, x);
                 if (d == 0 && a.lse) a.lse[(size_t)r * a.nh + h] = empty ? none : (top + log2f(sum)) * kLn2;
             }
         }

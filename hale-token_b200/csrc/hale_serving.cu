@@ -145,7 +145,7 @@ unsigned attn_grid(const hale_ctx* ctx, const KvArgs& c, const KvAttn& a, int pe
     return (unsigned)std::min<uint64_t>({(uint64_t)ctx->sm_count * per_sm, units, parts, (uint64_t)kAttnMaxGrid});
 }
 
-template <int DT, int DP, int NT>
+template <int DT, int DP, int HD, int NT>
 hale_status attn_few(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cudaStream_t st) {
     constexpr int cols = 8 * NT;
     a.heads = std::min(a.group, cols);
@@ -153,24 +153,30 @@ hale_status attn_few(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cud
     a.rows = (int)std::max<uint32_t>(1u, std::min<uint32_t>(run, (uint32_t)(cols / a.heads)));
     a.part_floats = cols * (2 + c.hd);
     const size_t smem = (size_t)kFewWarps * cols * DP * 4;
-    CUDA_TRY(ctx, allow_smem(kv_attn_few_kernel<DT, DP, NT>, smem));
+    CUDA_TRY(ctx, allow_smem(kv_attn_few_kernel<DT, DP, HD, NT>, smem));
     const unsigned grid = attn_grid(ctx, c, a, DP <= 128 && NT == 1 ? 3 : 2, FewCfg<DP>::CH);
-    kv_attn_few_kernel<DT, DP, NT><<<grid, kFewThreads, smem, st>>>(c, a);
+    kv_attn_few_kernel<DT, DP, HD, NT><<<grid, kFewThreads, smem, st>>>(c, a);
     return check_launch(ctx, "kv_attn_few");
-}
-
-template <int DT, int NT>
-hale_status attn_few_dim(hale_ctx* ctx, const KvArgs& c, const KvAttn& a, uint32_t run, cudaStream_t st) {
-    if (c.hd <= 64) return attn_few<DT, 64, NT>(ctx, c, a, run, st);
-    if (c.hd <= 128) return attn_few<DT, 128, NT>(ctx, c, a, run, st);
-    return attn_few<DT, 256, NT>(ctx, c, a, run, st);
 }
 
 template <int DT>
 hale_status attn_go(hale_ctx* ctx, const KvArgs& c, const KvAttn& a, uint32_t run, cudaStream_t st) {
     const uint64_t cols = (uint64_t)std::min<uint32_t>(run, (uint32_t)a.n) * a.group;
-    if (cols <= 8) return attn_few_dim<DT, 1>(ctx, c, a, run, st);
-    if (cols <= 16) return attn_few_dim<DT, 2>(ctx, c, a, run, st);
+    if (cols <= 8) {
+        switch (c.hd) {
+        case 64: return attn_few<DT, 64, 64, 1>(ctx, c, a, run, st);
+        case 128: return attn_few<DT, 128, 128, 1>(ctx, c, a, run, st);
+        case 256: return attn_few<DT, 256, 256, 1>(ctx, c, a, run, st);
+        default: return c.hd < 128 ? attn_few<DT, 128, 0, 1>(ctx, c, a, run, st) : attn_few<DT, 256, 0, 1>(ctx, c, a, run, st);
+        }
+    }
+    if (cols <= 16 && c.hd <= 128) {
+        switch (c.hd) {
+        case 64: return attn_few<DT, 64, 64, 2>(ctx, c, a, run, st);
+        case 128: return attn_few<DT, 128, 128, 2>(ctx, c, a, run, st);
+        default: return attn_few<DT, 128, 0, 2>(ctx, c, a, run, st);
+        }
+    }
     kv_attention_kernel<DT><<<dim3(a.n, a.nh), 128, 0, st>>>(c, a);
     return check_launch(ctx, "kv_attention");
 }

@@ -25,6 +25,8 @@
 // nothing of this is known when the kernel is launched.
 #pragma once
 
+#include <type_traits>
+
 #include "hale_kv.cuh"
 
 namespace hale {
@@ -244,12 +246,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Transposes an 8x8 matrix of 16-bit values held by a warp.
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -320,14 +316,15 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 // few columns: tokens x columns products fed from registers
 //
 // Four warps, each on its own 16 NB tokens of a unit. Keys: a lane loads 16
-// consecutive dims of two tokens, which are (after a permutation of the dims
-// that the query's fragment repeats) A fragments of 16 tokens x 32 dims as they
-// stand: nothing between HBM and the tensor core. S^T = K q^T leaves a column's
-// scores in the lanes of one quad position, so its weights, moved through an
-// 8x8 transpose, are the B fragment of O^T = V^T P^T, an f16 product (weights
-// span many orders of magnitude, which integers would cut off); V's A fragments
-// are again bytes of a lane's own loads (four tokens, DP / 8 consecutive dims),
-// paired by byte permutes and widened to f16.
+// consecutive dims of a token, which are (after a permutation of the dims that
+// the query's fragment repeats) B fragments of 32 dims x 8 tokens as they
+// stand: nothing between HBM and the tensor core. The A fragment's rows 0-7
+// hold the columns' highest digits and rows 8-15 the middle ones, so a lane
+// receives both sums of one column's score; a second product adds the lowest.
+// The scores lie so that the weights are the B fragment of O^T = V^T P^T, an
+// f16 product (weights span many orders of magnitude, which integers would cut
+// off); V's A fragments are again bytes of a lane's own loads (four tokens,
+// DP / 8 consecutive dims), paired by byte permutes and widened to f16.
 // Every load is made, hidden tokens and dims past the head's included (at an
 // address that is there): codes are finite whatever they are, and a hidden
 // token's weight, like a missing dim of q, is 0.
@@ -372,8 +369,8 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         // (the integer product's k index runs over 16 t + 4 q4 + byte of a
         // 32-dim step: words 0, 1 and 2, 3 of a lane's 16 dims)
         uint32_t qf[3][NT][KC * 2][2];
-        float qs[NT][2];
-        int end[NT][2], begin[NT][2];
+        float qs[NT];
+        int end[NT], begin[NT];
         int all_lo = 0, all_hi = INT_MAX;  // tokens every column sees
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -416,30 +413,25 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                     for (int z = 0; z < 3; z++) qf[z][nt][2 * p + (w >> 1)][w & 1] = d[z];
                 }
             if (wilds >> (4 * g) & 15u) up = __int_as_float(0x7fc00000);  // the column's scores become NaN
-            // the scores' columns are 2 q4 and 2 q4 + 1 of the lane
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int k = nt * 8 + 2 * q4 + e;
-                qs[nt][e] = a.scale * kLog2e / __shfl_sync(0xffffffffu, up, 8 * q4 + 4 * e);
-                end[nt][e] = begin[nt][e] = 0;
-                if (k < cols) {
-                    const int p = a.positions[seg.row + k / heads];
-                    end[nt][e] = p >= 0 && p < seg.hi ? p + 1 : 0;
-                    begin[nt][e] = a.window > 0 ? max(0, end[nt][e] - a.window) : 0;
-                    all_hi = min(all_hi, end[nt][e]);
-                    all_lo = max(all_lo, begin[nt][e]);
-                }
+            qs[nt] = a.scale * kLog2e / up;
+            end[nt] = begin[nt] = 0;
+            if (in) {
+                const int p = a.positions[seg.row + col / heads];
+                end[nt] = p >= 0 && p < seg.hi ? p + 1 : 0;
+                begin[nt] = a.window > 0 ? max(0, end[nt] - a.window) : 0;
+                all_hi = min(all_hi, end[nt]);
+                all_lo = max(all_lo, begin[nt]);
             }
         }
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
 
-        float acc[MT][NT][4], m[NT][2], l[NT][2];
+        float acc[MT][NT][4], m[NT], l[NT];
         float vtop = 0.0f, vinv = 0.0f;  // largest value scale so far, 2^14 over it
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = none;
-            l[nt][0] = l[nt][1] = 0.0f;
+            m[nt] = none;
+            l[nt] = 0.0f;
 #pragma unroll
             for (int i = 0; i < MT; i++) acc[i][nt][0] = acc[i][nt][1] = acc[i][nt][2] = acc[i][nt][3] = 0.0f;
         }
@@ -514,73 +506,70 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         load_k(u0, page, ks, vs);
         load_v(u0, page);
         find(u0 + 1, page_next);
-        for (int u = u0; u < u1; u++) {
+        // One step over the warp's tokens of unit u; WHOLE: every column sees
+        // all of them and every page is there.
+        auto step = [&](int u, auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
             const int t0 = u * CH + warp * Cfg::TB;
             const bool more = u + 1 < u1;
-            float s[NB][NT][4];  // q . kc as integers of at most 2^45, rounded to f32
+            // q . kc, integers of at most 2^45, rounded to f32; [token half][token]
+            float s[NB][NT][4];
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    int z0[4] = {0, 0, 0, 0}, z1[4] = {0, 0, 0, 0}, z2[4] = {0, 0, 0, 0};
+                for (int j = 0; j < 2; j++) {
+                    int z[NT][4], lo[(NT + 1) / 2][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0;
+#pragma unroll
+                    for (int i = 0; i < (NT + 1) / 2; i++) lo[i][0] = lo[i][1] = lo[i][2] = lo[i][3] = 0;
 #pragma unroll
                     for (int p = 0; p < KC; p++) {
-                        const uint4 x = kr[b][0][p], y = kr[b][1][p];
-                        mma_s8(z0, x.x, y.x, x.y, y.y, qf[0][nt][2 * p][0], qf[0][nt][2 * p][1]);
-                        mma_s8(z1, x.x, y.x, x.y, y.y, qf[1][nt][2 * p][0], qf[1][nt][2 * p][1]);
-                        mma_s8(z2, x.x, y.x, x.y, y.y, qf[2][nt][2 * p][0], qf[2][nt][2 * p][1]);
-                        mma_s8(z0, x.z, y.z, x.w, y.w, qf[0][nt][2 * p + 1][0], qf[0][nt][2 * p + 1][1]);
-                        mma_s8(z1, x.z, y.z, x.w, y.w, qf[1][nt][2 * p + 1][0], qf[1][nt][2 * p + 1][1]);
-                        mma_s8(z2, x.z, y.z, x.w, y.w, qf[2][nt][2 * p + 1][0], qf[2][nt][2 * p + 1][1]);
+                        const uint4 x = kr[b][j][p];
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            mma_s8(z[nt], qf[0][nt][2 * p][0], qf[1][nt][2 * p][0], qf[0][nt][2 * p][1], qf[1][nt][2 * p][1],
+                                   x.x, x.y);
+                            mma_s8(z[nt], qf[0][nt][2 * p + 1][0], qf[1][nt][2 * p + 1][0], qf[0][nt][2 * p + 1][1],
+                                   qf[1][nt][2 * p + 1][1], x.z, x.w);
+                        }
+#pragma unroll
+                        for (int i = 0; i < (NT + 1) / 2; i++) {  // the lowest digits of two sets of columns
+                            constexpr int last = NT - 1;
+                            const int n0 = 2 * i, n1 = NT == 1 ? 0 : (2 * i + 1 < last ? 2 * i + 1 : last);
+                            mma_s8(lo[i], qf[2][n0][2 * p][0], qf[2][n1][2 * p][0], qf[2][n0][2 * p][1], qf[2][n1][2 * p][1],
+                                   x.x, x.y);
+                            mma_s8(lo[i], qf[2][n0][2 * p + 1][0], qf[2][n1][2 * p + 1][0], qf[2][n0][2 * p + 1][1],
+                                   qf[2][n1][2 * p + 1][1], x.z, x.w);
+                        }
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; e++)  // |z| <= 2^22: z1 256 + z2 fits 32 bits
-                        s[b][nt][e] = fmaf((float)z0[e], 65536.0f, (float)(z1[e] * 256 + z2[e]));
-                }
-            if (more) load_k(u + 1, page_next, ks_next, vs_next);
-            // score = s f in units of log 2
-            float f[NB][NT][2];
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) f[b][nt][e] = ks[b] * qs[nt][e];
-            bool whole = t0 >= all_lo && t0 + Cfg::TB <= all_hi;
-#pragma unroll
-            for (int b = 0; b < NB; b++) whole = whole && page[b] >= 0;
-            unsigned hidden = 0;  // bit (b NT + nt) 4 + e
-            if (!whole) {
-#pragma unroll
-                for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int t = t0 + 16 * b + g + 8 * (e >> 1);
-                            if (page[b] < 0 || t >= end[nt][e & 1] || t < begin[nt][e & 1])
-                                hidden |= 1u << ((b * NT + nt) * 4 + e);
-                        }
-            }
-            float top[NT][2];
-            bool raise = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float x = m[nt][e];
-#pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        float y0 = s[b][nt][e] * f[b][nt][e], y1 = s[b][nt][e + 2] * f[b][nt][e];
-                        if (!whole) {
-                            y0 = hidden >> ((b * NT + nt) * 4 + e) & 1u ? none : y0;
-                            y1 = hidden >> ((b * NT + nt) * 4 + e + 2) & 1u ? none : y1;
-                        }
-                        x = fmaxf(x, fmaxf(y0, y1));
-                    }
-                    top[nt][e] = x;
-                    raise |= x > m[nt][e];
+                        for (int e = 0; e < 2; e++)  // sums of digits are at most 2^22: 256 mid + lo fits 32 bits
+                            s[b][nt][2 * j + e] = fmaf((float)z[nt][e], 65536.0f,
+                                                       (float)(z[nt][2 + e] * 256 + lo[nt / 2][2 * (nt & 1) + e]));
                 }
+            if (more) load_k(u + 1, page_next, ks_next, vs_next);
+            // score = s f in units of log 2
+            float f[NB][NT], top[NT];
+            bool hidden[NB][NT][4], raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                top[nt] = m[nt];
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    f[b][nt] = ks[b] * qs[nt];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int t = t0 + 16 * b + 8 * (e >> 1) + 2 * q4 + (e & 1);
+                        hidden[b][nt][e] = !WHOLE && (page[b] < 0 || t >= end[nt] || t < begin[nt]);
+                        const float y = s[b][nt][e] * f[b][nt];
+                        top[nt] = fmaxf(top[nt], hidden[b][nt][e] ? none : y);
+                    }
+                }
+                raise |= top[nt] > m[nt];
+            }
             float vmax = vtop;
 #pragma unroll
             for (int b = 0; b < NB; b++) vmax = fmaxf(vmax, vs[b]);
@@ -589,22 +578,24 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 vtop = vmax;
                 vinv = vmax > 0.0f ? kWeightTop / vmax : 0.0f;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++) {
+                    float x = top[nt];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    const float fix = m[nt] == none ? 0.0f : exp2_fast(m[nt] - x);
+                    m[nt] = x;
+                    l[nt] *= fix;
+                    // the outputs' columns are 2 q4 and 2 q4 + 1 of the lane
+                    const float fix0 = __shfl_sync(0xffffffffu, fix, 8 * q4) * fix_v;
+                    const float fix1 = __shfl_sync(0xffffffffu, fix, 8 * q4 + 4) * fix_v;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float x = top[nt][e];
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        const float fix = m[nt][e] == none ? 0.0f : exp2_fast(m[nt][e] - x), fix_acc = fix * fix_v;
-                        m[nt][e] = x;
-                        l[nt][e] *= fix;
-#pragma unroll
-                        for (int i = 0; i < MT; i++) {
-                            acc[i][nt][e] *= fix_acc;
-                            acc[i][nt][e + 2] *= fix_acc;
-                        }
+                    for (int i = 0; i < MT; i++) {
+                        acc[i][nt][0] *= fix0;
+                        acc[i][nt][1] *= fix1;
+                        acc[i][nt][2] *= fix0;
+                        acc[i][nt][3] *= fix1;
                     }
+                }
             }
             // weights, and V^T P^T
 #pragma unroll
@@ -613,23 +604,23 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 uint32_t pf[SPLIT][NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
+                    const float base = m[nt] == none ? 0.0f : m[nt];
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         // one rounding between the product and its distance from the maximum
-                        const float base = m[nt][e & 1] == none ? 0.0f : m[nt][e & 1];
-                        float p = exp2_fast(fmaf(s[b][nt][e], f[b][nt][e & 1], -base));
-                        if (!whole) p = hidden >> ((b * NT + nt) * 4 + e) & 1u ? 0.0f : p;
-                        l[nt][e & 1] += p;
+                        float p = exp2_fast(fmaf(s[b][nt][e], f[b][nt], -base));
+                        if (hidden[b][nt][e]) p = 0.0f;
+                        l[nt] += p;
                         w[e] = p * fv;
                     }
-                    pf[0][nt][0] = transpose8(pack_f16(w[0], w[1]));
-                    pf[0][nt][1] = transpose8(pack_f16(w[2], w[3]));
+                    pf[0][nt][0] = pack_f16(w[0], w[1]);
+                    pf[0][nt][1] = pack_f16(w[2], w[3]);
                     if (SPLIT == 2) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) w[e] -= __half2float(__float2half_rn(w[e]));
-                        pf[SPLIT - 1][nt][0] = transpose8(pack_f16(w[0], w[1]));
-                        pf[SPLIT - 1][nt][1] = transpose8(pack_f16(w[2], w[3]));
+                        pf[SPLIT - 1][nt][0] = pack_f16(w[0], w[1]);
+                        pf[SPLIT - 1][nt][1] = pack_f16(w[2], w[3]);
                     }
                 }
 #pragma unroll
@@ -657,23 +648,28 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 }
                 find(u + 2, page_next);
             }
+        };
+        for (int u = u0; u < u1; u++) {
+            const int t0 = u * CH + warp * Cfg::TB;
+            bool whole = t0 >= all_lo && t0 + Cfg::TB <= all_hi;
+#pragma unroll
+            for (int b = 0; b < NB; b++) whole = whole && page[b] >= 0;
+            if (whole) step(u, std::true_type{});
+            else step(u, std::false_type{});
         }
 
         // ---- the four warps' parts joined ----
         const float unscale = vtop / kWeightTop;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float x = l[nt][e];
-                x += __shfl_xor_sync(0xffffffffu, x, 4);
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (g == 0) {
-                    s_m[warp][nt * 8 + 2 * q4 + e] = m[nt][e];
-                    s_l[warp][nt * 8 + 2 * q4 + e] = x;
-                }
+        for (int nt = 0; nt < NT; nt++) {
+            float x = l[nt];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            if (q4 == 0) {
+                s_m[warp][nt * 8 + g] = m[nt];
+                s_l[warp][nt * 8 + g] = x;
             }
+        }
         __syncthreads();
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -684,11 +680,11 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
 #pragma unroll
                 for (int w = 1; w < kFewWarps; w++) top = fmaxf(top, s_m[w][k]);
                 // (a part that saw nothing is 0, or NaN where its scores were)
-                const float f = (m[nt][e] == none ? 1.0f : exp2_fast(m[nt][e] - top)) * unscale;
+                const float mine = s_m[warp][k], fw = (mine == none ? 1.0f : exp2_fast(mine - top)) * unscale;
                 float* dst = s_acc + ((size_t)warp * COLS + k) * DP + 4 * VW * g;
 #pragma unroll
                 for (int i = 0; i < MT; i++)
-                    *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][nt][e] * f, acc[i][nt][e + 2] * f);
+                    *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][nt][e] * fw, acc[i][nt][e + 2] * fw);
             }
         if (tid < COLS) {
             float top = s_m[0][tid], sum = 0.0f;

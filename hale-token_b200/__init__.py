@@ -597,39 +597,58 @@ def sample(ctx, logits, params, rng_state, out_tokens, seen_ids=None, stream=Non
              _stream(stream))
 
 
+_DTYPE_CODES = {}
+
+
 def _dtype_code(t, what):
-    import torch
-    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    if not _DTYPE_CODES:
+        import torch
+        _DTYPE_CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    code = _DTYPE_CODES.get(t.dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
     return code
 
 
-def _on(ctx, stream, **tensors):
+def _on(ctx, stream, *tensors):
     """Checks that the tensors are on ctx's GPU; the stream handle to use: the
     given one, or torch's current stream of ctx's GPU."""
-    import torch
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != ctx.device):
-            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    dev = ctx.device
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, the context on cuda:{dev}")
     if stream is None:
-        return C.c_void_p(torch.cuda.current_stream(ctx.device).cuda_stream)
-    return _stream(stream)
+        import torch
+        return torch.cuda.current_stream(dev).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _ints(t, shape, name):
+def _at(t):
+    """Address of a tensor (or None) for a c_void_p argument."""
+    return None if t is None else t.data_ptr()
+
+
+def _ints(t, n, name):
+    """A contiguous int32 vector of n."""
     import torch
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}], not {t.dtype} {tuple(t.shape)}")
+
+
+def _shaped(t, dtype, shape, name):
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
 
 
 def _row_stride(t, heads, dim, name):
     """Row stride of [n, heads, dim] with whole rows (rows may lie apart)."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} must be [rows, {heads}, {dim}], not {tuple(t.shape)}")
-    if t.shape[0] and ((dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim)):
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name} must be [rows, {heads}, {dim}], not {tuple(shape)}")
+    rows, head, one = t.stride()
+    if shape[0] and ((dim > 1 and one != 1) or (heads > 1 and head != dim)):
         raise ValueError(f"the values of a row of {name} must lie together")
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+    return rows if shape[0] > 1 else heads * dim
 
 
 class Kv8:
@@ -651,15 +670,14 @@ class Kv8:
         if k.dim() != 5 or table.dim() != 2:
             raise ValueError("k must be [layers, pages, kv heads, page tokens, head dim], table [sequences, pages]")
         L, n_pages, nkv, pt, hd = k.shape
-        wants = dict(k=(k, k.shape, torch.int8), v=(v, k.shape, torch.int8),
-                     k_scale=(k_scale, (L, n_pages, nkv, pt // 16), torch.float32),
-                     v_scale=(v_scale, (L, n_pages, nkv, pt // 16), torch.float32),
-                     table=(table, table.shape, torch.int32), lens=(lens, (table.shape[0],), torch.int32),
-                     refs=(refs, (n_pages,), torch.int32))
-        for name, (t, shape, dt) in wants.items():
-            if t.dtype != dt or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous {dt} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
-        _on(ctx, 0, k=k, v=v, k_scale=k_scale, v_scale=v_scale, table=table, lens=lens, refs=refs)
+        _shaped(k, torch.int8, k.shape, "k")
+        _shaped(v, torch.int8, k.shape, "v")
+        _shaped(k_scale, torch.float32, (L, n_pages, nkv, pt // 16), "k_scale")
+        _shaped(v_scale, torch.float32, (L, n_pages, nkv, pt // 16), "v_scale")
+        _shaped(table, torch.int32, table.shape, "table")
+        _ints(lens, table.shape[0], "lens")
+        _ints(refs, n_pages, "refs")
+        _on(ctx, 0, k, v, k_scale, v_scale, table, lens, refs)
         self.ctx = ctx
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.table, self.lens, self.refs = table, lens, refs
@@ -683,25 +701,30 @@ class Kv8:
                    torch.zeros(n_pages, dtype=torch.int32, device=dev))
 
     def _rows(self, n, positions, seqs):
-        _ints(positions, (n,), "positions")
+        _ints(positions, n, "positions")
         if seqs is not None:
-            _ints(seqs, (n,), "seqs")
+            _ints(seqs, n, "seqs")
+
+    def _call(self, fn, *args):
+        status = fn(self.ctx.h, self._ref, *args)
+        if status != OK:
+            _check(status, self.ctx.h)
 
     def append(self, layer, k, v, positions, seqs=None, stream=None):
         """hale_kv8_append: rows k, v [n, kv heads, head dim] become tokens
         positions[r] of sequences seqs[r]."""
-        st = _on(self.ctx, stream, k=k, v=v, positions=positions, seqs=seqs)
+        st = _on(self.ctx, stream, k, v, positions, seqs)
         self._rows(k.shape[0], positions, seqs)
-        if v.dtype != k.dtype or v.shape != k.shape:
+        if v.dtype is not k.dtype or v.shape != k.shape:
             raise ValueError("k and v must have one type and shape")
-        self.ctx.call("hale_kv8_append", self.ctx.h, self._ref, layer, ptr(k), ptr(v), _dtype_code(k, "k"),
-                      _row_stride(k, self.n_kv_heads, self.head_dim, "k"),
-                      _row_stride(v, self.n_kv_heads, self.head_dim, "v"), ptr(seqs), ptr(positions), k.shape[0], st)
+        self._call(lib().hale_kv8_append, layer, k.data_ptr(), v.data_ptr(), _dtype_code(k, "k"),
+                   _row_stride(k, self.n_kv_heads, self.head_dim, "k"),
+                   _row_stride(v, self.n_kv_heads, self.head_dim, "v"), _at(seqs), positions.data_ptr(), k.shape[0], st)
 
     def read(self, layer, k_out, v_out, positions, seqs=None, stream=None):
         """hale_kv8_read: tokens as the values the cache stands for; either
         output may be None."""
-        st = _on(self.ctx, stream, k_out=k_out, v_out=v_out, positions=positions, seqs=seqs)
+        st = _on(self.ctx, stream, k_out, v_out, positions, seqs)
         some = [t for t in (k_out, v_out) if t is not None]
         if not some:
             return
@@ -711,51 +734,56 @@ class Kv8:
                    for t in (k_out, v_out)]
         for t in some:
             self._rows(t.shape[0], positions, seqs)
-        self.ctx.call("hale_kv8_read", self.ctx.h, self._ref, layer, ptr(seqs), ptr(positions), some[0].shape[0],
-                      ptr(k_out), ptr(v_out), _dtype_code(some[0], "k_out / v_out"), *strides, st)
+        self._call(lib().hale_kv8_read, layer, _at(seqs), positions.data_ptr(), some[0].shape[0], _at(k_out), _at(v_out),
+                   _dtype_code(some[0], "k_out / v_out"), *strides, st)
 
     def attention(self, layer, q, out, positions, seqs=None, scale=None, window=0, run=1, lse=None, stream=None):
         """hale_kv8_attention: q, out [n, heads, head dim]; lse float32
         [n, heads] or None; scale None is head_dim ** -0.5."""
-        import torch
-        st = _on(self.ctx, stream, q=q, out=out, positions=positions, seqs=seqs, lse=lse)
-        self._rows(q.shape[0], positions, seqs)
-        if out.dtype != q.dtype or out.shape != q.shape:
-            raise ValueError("q and out must have one type and shape")
-        heads = q.shape[1] if q.dim() == 3 else 0
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
-            raise ValueError(f"lse must be contiguous float32 {tuple(q.shape[:2])}")
-        self.ctx.call("hale_kv8_attention", self.ctx.h, self._ref, layer, ptr(q), _dtype_code(q, "q"),
-                      _row_stride(q, heads, self.head_dim, "q"), ptr(seqs), ptr(positions), q.shape[0], heads,
-                      self.head_dim ** -0.5 if scale is None else scale, window, run, ptr(out),
-                      _row_stride(out, heads, self.head_dim, "out"), ptr(lse), st)
+        st = _on(self.ctx, stream, q, out, positions, seqs, lse)
+        shape = q.shape
+        if len(shape) != 3 or out.dtype is not q.dtype or out.shape != shape:
+            raise ValueError("q and out must be [rows, heads, head dim] of one type")
+        n, heads, dim = shape
+        self._rows(n, positions, seqs)
+        if lse is not None:
+            import torch
+            _shaped(lse, torch.float32, (n, heads), "lse")
+        self._call(lib().hale_kv8_attention, layer, q.data_ptr(), _dtype_code(q, "q"),
+                   _row_stride(q, heads, self.head_dim, "q"), _at(seqs), positions.data_ptr(), n, heads,
+                   self.head_dim ** -0.5 if scale is None else scale, window, run, out.data_ptr(),
+                   _row_stride(out, heads, self.head_dim, "out"), _at(lse), st)
 
     def resize(self, new_lens, seqs=None, stream=None):
         """hale_kv8_resize: sequence seqs[i] (None: i) gets length new_lens[i]."""
-        st = _on(self.ctx, stream, new_lens=new_lens, seqs=seqs)
-        self._rows(new_lens.shape[0], new_lens, seqs)
-        self.ctx.call("hale_kv8_resize", self.ctx.h, self._ref, ptr(seqs), ptr(new_lens), new_lens.shape[0], st)
+        st = _on(self.ctx, stream, new_lens, seqs)
+        n = new_lens.shape[0]
+        self._rows(n, new_lens, seqs)
+        self._call(lib().hale_kv8_resize, _at(seqs), new_lens.data_ptr(), n, st)
 
     def fork(self, parents, children, stream=None):
         """hale_kv8_fork: children[i] becomes a copy of parents[i] that shares its pages."""
-        st = _on(self.ctx, stream, parents=parents, children=children)
-        _ints(parents, parents.shape[:1], "parents")
-        _ints(children, parents.shape, "children")
-        self.ctx.call("hale_kv8_fork", self.ctx.h, self._ref, ptr(parents), ptr(children), parents.shape[0], st)
+        st = _on(self.ctx, stream, parents, children)
+        n = parents.shape[0]
+        _ints(parents, n, "parents")
+        _ints(children, n, "children")
+        self._call(lib().hale_kv8_fork, parents.data_ptr(), children.data_ptr(), n, st)
 
     def compact(self, remap, live, stream=None):
         """hale_kv8_compact: remap int32 [2, pages], live int32 [1]."""
-        st = _on(self.ctx, stream, remap=remap, live=live)
-        _ints(remap, (2, self.n_pages), "remap")
-        _ints(live, (1,), "live")
-        self.ctx.call("hale_kv8_compact", self.ctx.h, self._ref, ptr(remap), ptr(live), st)
+        import torch
+        st = _on(self.ctx, stream, remap, live)
+        _shaped(remap, torch.int32, (2, self.n_pages), "remap")
+        _ints(live, 1, "live")
+        self._call(lib().hale_kv8_compact, remap.data_ptr(), live.data_ptr(), st)
 
     def copy_pages(self, src, dst, stream=None):
         """hale_kv8_copy: pages src[i] -> dst[i] of every layer."""
-        st = _on(self.ctx, stream, src=src, dst=dst)
-        _ints(src, src.shape[:1], "src")
-        _ints(dst, src.shape, "dst")
-        self.ctx.call("hale_kv8_copy", self.ctx.h, self._ref, ptr(src), ptr(dst), src.shape[0], st)
+        st = _on(self.ctx, stream, src, dst)
+        n = src.shape[0]
+        _ints(src, n, "src")
+        _ints(dst, n, "dst")
+        self._call(lib().hale_kv8_copy, src.data_ptr(), dst.data_ptr(), n, st)
 
 
 def verify_drafts(ctx, logits, draft_tokens, uniforms, out_tokens, out_n, draft_probs=None, n_draft=None,
@@ -766,33 +794,38 @@ def verify_drafts(ctx, logits, draft_tokens, uniforms, out_tokens, out_n, draft_
     None; out_tokens int32 [batch, max_draft + 1], out_n int32 [batch],
     out_logp float32 like out_tokens or None."""
     import torch
-    st = _on(ctx, stream, logits=logits, draft_tokens=draft_tokens, uniforms=uniforms, out_tokens=out_tokens,
-             out_n=out_n, draft_probs=draft_probs, n_draft=n_draft, out_logp=out_logp)
+    st = _on(ctx, stream, logits, draft_tokens, uniforms, out_tokens, out_n, draft_probs, n_draft, out_logp)
 
-    def rows(t, name):  # rows of one tensor lie a fixed stride apart
-        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1) or (
-                t.shape[0] > 1 and t.shape[1] > 0 and t.stride(0) != t.shape[1] * t.stride(1)):
-            raise ValueError(f"{name} must be [batch, rows, vocab] with rows a fixed stride apart")
-        return max(t.stride(1), t.shape[2])
+    def rows(t, name):  # stride of a tensor's rows, which lie a fixed distance apart
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [batch, rows, vocab]")
+        many, row, one = t.stride()
+        batch, n, width = t.shape
+        if (width > 1 and one != 1) or (batch > 1 and n > 1 and many != n * row):
+            raise ValueError(f"the rows of {name} must lie a fixed distance apart")
+        return max(row if n > 1 else many if batch > 1 else width, width)
 
     stride = rows(logits, "logits")
     B, R, V = logits.shape
-    _ints(draft_tokens, (B, R - 1), "draft_tokens")
-    _ints(out_tokens, (B, R), "out_tokens")
-    _ints(out_n, (B,), "out_n")
+    _shaped(draft_tokens, torch.int32, (B, R - 1), "draft_tokens")
+    _shaped(out_tokens, torch.int32, (B, R), "out_tokens")
+    _ints(out_n, B, "out_n")
     if n_draft is not None:
-        _ints(n_draft, (B,), "n_draft")
-    for name, t in (("uniforms", uniforms), ("out_logp", out_logp)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, R) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 {(B, R)}")
+        _ints(n_draft, B, "n_draft")
+    if uniforms is not None:
+        _shaped(uniforms, torch.float32, (B, R), "uniforms")
+    if out_logp is not None:
+        _shaped(out_logp, torch.float32, (B, R), "out_logp")
     pstride = 0
     if draft_probs is not None:
-        if draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (B, R - 1, V):
+        if draft_probs.dtype is not torch.float32 or draft_probs.shape != (B, R - 1, V):
             raise ValueError(f"draft_probs must be float32 {(B, R - 1, V)}")
         pstride = rows(draft_probs, "draft_probs")
-    ctx.call("hale_verify_drafts", ctx.h, ptr(logits), _dtype_code(logits, "logits"), stride, ptr(draft_tokens),
-             ptr(draft_probs), pstride, ptr(n_draft), B, R - 1, V, temperature, ptr(uniforms), ptr(out_tokens),
-             ptr(out_n), ptr(out_logp), st)
+    status = lib().hale_verify_drafts(
+        ctx.h, logits.data_ptr(), _dtype_code(logits, "logits"), stride, draft_tokens.data_ptr(), _at(draft_probs), pstride,
+        _at(n_draft), B, R - 1, V, temperature, _at(uniforms), out_tokens.data_ptr(), out_n.data_ptr(), _at(out_logp), st)
+    if status != OK:
+        _check(status, ctx.h)
 
 
 def row_bytes(dtype, cols):

@@ -166,17 +166,6 @@ __global__ void qk_rope_kernel(float* __restrict__ qkv, int nh, int nkv, int hd,
     }
 }
 
-// 16-byte asynchronous global -> shared copies (cp.async, sm_80+).
-__device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
-    const unsigned sa = (unsigned)__cvta_generic_to_shared(smem);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(sa), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
-
 // Attention's V staging: kAttnStages stages of attn_v_rows(hd) positions
 // (16 KB each).
 constexpr int kAttnStages = 3;

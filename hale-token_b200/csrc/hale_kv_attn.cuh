@@ -19,10 +19,12 @@
 // `rows` consecutive rows of one sequence; a tile is a segment with one kv
 // head (its rows and the head's query heads are the tile's columns); a unit is
 // one chunk of the tile's tokens. The units of all tiles, in order, are dealt
-// out evenly: CTA c of G takes units [c W / G, (c + 1) W / G). A tile that
-// falls into several CTAs is joined by the last of them to finish, in CTA
-// order, so results do not depend on timing. Lengths are read on the device:
-// nothing of this is known when the kernel is launched.
+// out evenly over the CTAs. A tile that falls into several CTAs leaves its
+// parts in the workspace, and a second, small kernel joins them in CTA order,
+// so results do not depend on timing. (Joined by the last CTA to arrive, a
+// tile's parts cost the same kernel a fence, a counter and 100 registers of
+// its token loop.) Lengths are read on the device: nothing of this is known
+// when the kernels are launched.
 #pragma once
 
 #include <type_traits>
@@ -30,6 +32,12 @@
 #include "hale_kv.cuh"
 
 namespace hale {
+
+// A tile whose parts lie in the workspace: parts of CTAs c .. c + parts - 1
+// (parts 0: none begins in CTA c).
+struct KvSplit {
+    int parts, cols, heads, row, h0;
+};
 
 struct KvAttn {
     const void* q;
@@ -44,7 +52,7 @@ struct KvAttn {
     float scale;
     float* parts;        // [2 * gridDim][part_floats]
     int part_floats;
-    unsigned* arrived;   // [gridDim], zero between calls
+    KvSplit* splits;     // [gridDim] the tile that begins in each CTA and is not finished there
 };
 
 // Workspace of split tiles.
@@ -54,8 +62,15 @@ constexpr int kAttnMaxGrid = 1024;
 struct KvSegment {
     int row, rows, seq;
     int lo, hi;      // tokens any of its rows sees: [lo, hi)
-    int c0, units;   // first chunk and number of chunks
+    int c0, units;   // first chunk; chunks, and kTileCost units more
 };
+
+// What beginning and ending a tile costs, in units (preparing queries, joining
+// warps: 4 us, where a unit of 128 tokens takes 2.5 us): a tile's first
+// kTileCost units stand for it and hold no tokens, so that a CTA with many
+// short tiles gets fewer tokens. Without them 64 sequences of up to 8191
+// tokens took 138 us, CTAs with 12 tiles ending at 137, the median at 101.
+constexpr int kTileCost = 2;
 
 // One past the last token row i sees, 0 for a row that sees nothing.
 __device__ __forceinline__ int kv_row_end(const KvArgs& c, const KvAttn& a, int i, int seq) {
@@ -91,60 +106,66 @@ __device__ __forceinline__ KvSegment kv_segment(const KvArgs& c, const KvAttn& a
     if (s.hi == 0) s.lo = 0;
     s.c0 = s.lo / CH;
     // a segment that sees nothing is still one unit: its rows are written
-    s.units = max(1, (s.hi + CH - 1) / CH - s.c0);
+    s.units = max(1, (s.hi + CH - 1) / CH - s.c0) + kTileCost;
     return s;
 }
 
-// The units a CTA owns, walked segment by segment.
+// The units a CTA owns, walked segment by segment: of `total` units CTA c gets
+// `each`, the first `extra` CTAs one more. Units are counted in 32 bits (the
+// host cuts calls that could have more into several).
 template <int CH, int THREADS>
 struct KvWalk {
-    long long total, begin, end;  // units of all tiles; this CTA's
-    int grid;                     // CTAs that have units
-    long long base;               // units before the current segment
+    unsigned begin, end;   // this CTA's units
+    unsigned each, extra;
+    unsigned base;         // units before the current segment
     KvSegment seg;
 
-    __device__ __forceinline__ int owner(long long unit) const { return (int)(((unit + 1) * grid - 1) / total); }
+    __device__ __forceinline__ unsigned owner(unsigned unit) const {
+        const unsigned big = extra * (each + 1);
+        return unit < big ? unit / (each + 1) : extra + (unit - big) / each;
+    }
 
     // All threads. False: nothing to do.
-    __device__ bool start(const KvArgs& c, const KvAttn& a, KvSegment* s_seg, long long* s_sum) {
+    __device__ bool start(const KvArgs& c, const KvAttn& a, KvSegment* s_seg, unsigned* s_sum) {
         constexpr int W = THREADS / 32;
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
         const int tiles = c.nkv * a.subs;
         const int strip = (a.n + THREADS - 1) / THREADS, i0 = tid * strip, i1 = min(a.n, i0 + strip);
-        long long mine = 0;
+        unsigned mine = 0;
         KvSegment first;
         first.rows = 0;
         for (int i = i0; i < i1; i++) {
             const KvSegment s = kv_segment<CH>(c, a, i);
-            if (s.rows) mine += (long long)s.units * tiles;
+            if (s.rows) mine += (unsigned)(s.units * tiles);
             if (s.rows && !first.rows) first = s;
         }
-        long long x = mine;
+        unsigned x = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
         if (lane == 31) s_sum[warp] = x;
         __syncthreads();
-        total = 0;
-        long long before = 0;
+        unsigned total = 0, before = 0;
 #pragma unroll
         for (int w = 0; w < W; w++) {
             if (w < warp) before += s_sum[w];
             total += s_sum[w];
         }
-        grid = (int)min((long long)gridDim.x, total);
-        if ((int)blockIdx.x >= grid) return false;
-        begin = total * blockIdx.x / grid;
-        end = total * (blockIdx.x + 1) / grid;
+        if (blockIdx.x >= total) return false;
+        const unsigned grid = min(gridDim.x, total);
+        each = total / grid;
+        extra = total - each * grid;
+        begin = blockIdx.x * each + min(blockIdx.x, extra);
+        end = begin + each + (blockIdx.x < extra);
         before += x - mine;
         if (begin >= before && begin < before + mine) {
             // this thread's strip holds the first unit
             for (int i = first.row;; i++) {
                 const KvSegment s = i == first.row ? first : kv_segment<CH>(c, a, i);
                 if (!s.rows) continue;
-                const long long u = (long long)s.units * tiles;
+                const unsigned u = (unsigned)(s.units * tiles);
                 if (begin < before + u) {
                     *s_seg = s;
                     s_sum[W] = before;
@@ -161,7 +182,7 @@ struct KvWalk {
 
     // The next segment with units (there is one while base < end).
     __device__ void next(const KvArgs& c, const KvAttn& a) {
-        base += (long long)seg.units * c.nkv * a.subs;
+        base += (unsigned)(seg.units * c.nkv * a.subs);
         int i = seg.row + seg.rows;
         while (i < a.n) {
             seg = kv_segment<CH>(c, a, i);
@@ -242,9 +263,19 @@ __global__ void __launch_bounds__(128) kv_attention_kernel(KvArgs c, KvAttn a) {
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 load_shared8(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -263,20 +294,6 @@ __device__ __forceinline__ uint32_t codes_even(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return codes_even(w >> 8); }
-
-// 16 (or 8) bytes that no one else will read again soon.
-__device__ __forceinline__ uint4 load_stream16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 load_stream8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
 
 constexpr float kWeightTop = 16384.0f;  // the largest weight as f16
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -305,11 +322,89 @@ __device__ __forceinline__ void kv_query_digits(const float (&x)[4], uint32_t (&
     }
 }
 
+// d = a b, or d += a b.
+template <bool FIRST>
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (FIRST)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four dims of a row's result from the weighted sum x, the maximum and the sum
+// of its weights; its lse beside the first.
+template <int DT>
+__device__ __forceinline__ void kv_finish(const KvAttn& a, int row, int head, int hd, int d, float (&x)[4], float top,
+                                          float sum) {
+    const float none = -__int_as_float(0x7f800000);
+    const bool empty = top == none && sum == 0.0f;  // nothing seen (not: NaN scores, whose sum is NaN)
+    const float inv = empty ? 0.0f : __fdiv_rn(1.0f, sum);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = empty ? 0.0f : x[e] * inv;
+    store4<DT>(a.out, (size_t)row * a.out_stride + (size_t)head * hd + d, x);
+    if (d == 0 && a.lse) a.lse[(size_t)row * a.nh + head] = empty ? none : (top + log2f(sum)) * kLn2;
+}
+
+// Split tiles joined, in CTA order: one CTA per possible tile, a warp per
+// column, lanes over the dims; what a part counts is computed by the lanes
+// over the parts while the first eight parts' values are under way.
+constexpr int kJoinThreads = 256;
+
+template <int DT>
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(KvAttn a, int hd, int max_cols) {
+    constexpr int BATCH = 8;
+    const int lane = threadIdx.x & 31, c = blockIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const KvSplit t = a.splits[c];
+    if (t.parts == 0) return;
+    const float none = -__int_as_float(0x7f800000);
+    const float* base = a.parts + (size_t)2 * c * a.part_floats;
+    auto part = [&](int r) { return base + (size_t)(2 * r + (r == 0)) * a.part_floats; };
+    for (int k = threadIdx.x >> 5; k < t.cols; k += kJoinThreads / 32) {
+        for (int d = 4 * lane; d < (hd + 127) / 128 * 128; d += 128) {
+            float4 y[BATCH];
+            const bool in = d < hd;
+            const size_t at = 2 * max_cols + (size_t)k * hd + d;
+#pragma unroll
+            for (int r = 0; r < BATCH; r++)
+                y[r] = in && r < t.parts ? *reinterpret_cast<const float4*>(part(r) + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float top = none, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = lane; r < t.parts; r += 32) top = fmaxf(top, part(r)[k]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int r0 = 0; r0 < t.parts; r0 += 32) {
+                const int r = r0 + lane;
+                float w = 0.0f;
+                if (r < t.parts) {
+                    const float m = part(r)[k];
+                    w = m == none ? 1.0f : exp2_fast(m - top);  // (a part that saw nothing is 0)
+                    sum = fmaf(w, part(r)[max_cols + k], sum);
+                }
+                for (int i0 = 0; i0 < 32 && r0 + i0 < t.parts; i0 += BATCH) {
+                    if (r0 + i0 > 0) {
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++)
+                            y[i] = in && r0 + i0 + i < t.parts ? *reinterpret_cast<const float4*>(part(r0 + i0 + i) + at)
+                                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) {
+                        const float f = __shfl_sync(0xffffffffu, w, i0 + i);
+                        x[0] = fmaf(f, y[i].x, x[0]); x[1] = fmaf(f, y[i].y, x[1]);
+                        x[2] = fmaf(f, y[i].z, x[2]); x[3] = fmaf(f, y[i].w, x[3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (in) kv_finish<DT>(a, t.row + k / t.heads, t.h0 + k % t.heads, hd, d, x, top, sum);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -325,8 +420,12 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 // f16 product (weights span many orders of magnitude, which integers would cut
 // off); V's A fragments are again bytes of a lane's own loads (four tokens,
 // DP / 8 consecutive dims), paired by byte permutes and widened to f16.
-// Every load is made, hidden tokens and dims past the head's included (at an
-// address that is there): codes are finite whatever they are, and a hidden
+// Codes reach a warp through its own ring of stages in shared memory, filled
+// by 16-byte asynchronous copies STAGES - 1 steps ahead: a warp waits for no
+// other, and the bytes in flight do not depend on where its arithmetic stands.
+// A token's 16-byte pieces are permuted (xor with bits of the token's number)
+// so that the fragments' loads meet no bank twice. Whatever bytes lie in a
+// hidden token or behind the head's dims, they are finite codes, and the
 // token's weight, like a missing dim of q, is 0.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 
@@ -334,8 +433,30 @@ template <int DP>
 struct FewCfg {
     static constexpr int NB = DP <= 128 ? 2 : 1;         // blocks of 16 tokens a warp takes at a time
     static constexpr int TB = 16 * NB, CH = TB * kFewWarps;
+    static constexpr int STAGES = 2;
+    static constexpr int STAGE = 2 * TB * DP;            // bytes of a stage: keys, then values
+    static constexpr int RING = STAGES * STAGE;          // of one warp
+    static constexpr int PIECES = DP / 16;               // 16-byte pieces of a row
     static constexpr int KC = DP / 64;                   // 64-dim pieces of a key row
     static constexpr int VW = DP / 32;                   // 32-bit words of a lane's dims of one value row
+};
+
+// Where a token's piece i goes: i ^ swizzle. A key load reads pieces 4 p + 0..3
+// of tokens g, g + 1: with 128-byte rows odd tokens move to the other half. A
+// value load reads piece g of tokens 0, 2, 4, 6 (and g + 1 beside it).
+template <int DP>
+__device__ __forceinline__ int few_key_swizzle(int t) {
+    return DP >= 128 ? (t & 1) << 2 : 0;
+}
+template <int DP>
+__device__ __forceinline__ int few_value_swizzle(int t) {
+    return DP >= 128 ? (t >> 1 & 3) << 1 : t >> 1 & 3;
+}
+
+// A block in a stage: its scales and its page (-1: nothing of it is seen).
+struct alignas(16) FewBlock {
+    float ks, vs;
+    int page, unused;
 };
 
 // HD: the head's dims where they are known (= DP), else 0.
@@ -345,80 +466,166 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
     constexpr int NB = Cfg::NB, CH = Cfg::CH, KC = Cfg::KC, VW = Cfg::VW, MT = DP / 16, COLS = 8 * NT;
     constexpr int SPLIT = DT == 0 ? 2 : 1;
     __shared__ KvSegment s_seg;
-    __shared__ long long s_sum[kFewWarps + 1];
+    __shared__ unsigned s_sum[kFewWarps + 1];
     __shared__ float s_m[kFewWarps][COLS], s_l[kFewWarps][COLS], s_f[COLS], s_inv[COLS];
-    __shared__ int s_last;
-    extern __shared__ __align__(16) float s_acc[];  // [kFewWarps][COLS][DP]
+    __shared__ __align__(16) int8_t s_q[3][COLS][DP + 16];
+    __shared__ int s_end[COLS];
+    __shared__ FewBlock s_block[kFewWarps][Cfg::STAGES][NB];
+    extern __shared__ __align__(128) int8_t s_ring[];  // [kFewWarps][RING]; between tiles the warps' sums
+    float* s_acc = reinterpret_cast<float*>(s_ring);   // [kFewWarps][COLS][DP]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+    const uint32_t ring = smem_addr(s_ring) + warp * Cfg::RING;
     const int hd = HD ? HD : c.hd;
     const float none = -__int_as_float(0x7f800000);
 
+    if (tid == 0) a.splits[blockIdx.x].parts = 0;
     KvWalk<CH, kFewThreads> walk;
     if (!walk.start(c, a, &s_seg, s_sum)) return;
-    long long unit = walk.begin;
+    unsigned unit = walk.begin;
     while (unit < walk.end) {
-        while (unit >= walk.base + (long long)walk.seg.units * c.nkv * a.subs) walk.next(c, a);
+        while (unit >= walk.base + (unsigned)(walk.seg.units * c.nkv * a.subs)) walk.next(c, a);
         const KvSegment seg = walk.seg;
-        const int tile = (int)((unit - walk.base) / seg.units), head = tile / a.subs, sub = tile % a.subs;
-        const long long tile0 = walk.base + (long long)tile * seg.units, tile1 = tile0 + seg.units;
-        const int u0 = seg.c0 + (int)(unit - tile0), u1 = seg.c0 + (int)(min(tile1, walk.end) - tile0);
+        const int tile = (int)((unit - walk.base) / (unsigned)seg.units), head = tile / a.subs, sub = tile - head * a.subs;
+        const unsigned tile0 = walk.base + (unsigned)(tile * seg.units), tile1 = tile0 + seg.units;
+        const unsigned first = tile0 + kTileCost;  // the tile's first chunk
+        if (walk.end <= first) return;             // this CTA's units end before it
+        const unsigned from = max(unit, first);
+        const int u0 = seg.c0 + (int)(from - first), u1 = seg.c0 + (int)(min(tile1, walk.end) - first);
         const int heads = min(a.heads, a.group - sub * a.heads), cols = seg.rows * heads;
         const int h0 = head * a.group + sub * a.heads;  // the tile's first query head
 
-        // ---- the columns' queries, as B fragments, and what they see ----
-        // (the integer product's k index runs over 16 t + 4 q4 + byte of a
-        // 32-dim step: words 0, 1 and 2, 3 of a lane's 16 dims)
+        // ---- the first tokens are under way while the queries are prepared ----
+        const int32_t* row = c.table + (size_t)min(seg.seq, c.n_seqs - 1) * c.max_pages;
+        // a page's codes (at most 2^26 bytes) and scales
+        const unsigned page_codes = (unsigned)(c.nkv * hd) << c.page_log2, page_scales = (unsigned)c.nkv << c.page_log2 >> 4;
+        // this lane's pieces: 32 / PIECES rows apart
+        constexpr int PIECES = Cfg::PIECES, ROWS = 32 / PIECES;
+        const int my_row = lane / PIECES, my_piece = lane % PIECES;
+        const size_t my_at = ((size_t)head << c.page_log2) * hd + (unsigned)(my_row * hd + 16 * my_piece);
+        const bool copies = HD || 16 * my_piece < hd;
+        // (the swizzles are linear in a token's bits, and my_row and the steps share none)
+        const uint32_t key_to = my_row * DP + 16 * (my_piece ^ few_key_swizzle<DP>(my_row));
+        const uint32_t value_to = my_row * DP + 16 * (my_piece ^ few_value_swizzle<DP>(my_row));
+        // where the fragments' tokens g and 2 q4 lie
+        const uint32_t key_at[2] = {(uint32_t)(g * DP + 16 * (q4 ^ few_key_swizzle<DP>(g))),
+                                    (uint32_t)(g * DP + 16 * ((4 + q4) ^ few_key_swizzle<DP>(g)))};
+        const uint32_t value_at = 2 * q4 * DP + (VW == 2 ? 16 * ((g >> 1) ^ few_value_swizzle<DP>(2 * q4)) + 8 * (g & 1)
+                                                         : 16 * ((VW / 4 * g) ^ few_value_swizzle<DP>(2 * q4)));
+        const float* ksbase = c.ks + ((size_t)head << c.page_log2 >> 4);
+        const float* vsbase = c.vs + ((size_t)head << c.page_log2 >> 4);
+
+        // page of each block of unit u, -1: nothing of it is seen, or it is missing
+        int page_next[NB];
+        auto find = [&](int u) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const int t = u * CH + warp * Cfg::TB + 16 * b;
+                page_next[b] = -1;
+                if (u < u1 && t < seg.hi && t + 16 > seg.lo) {
+                    page_next[b] = c.checked(row[t >> c.page_log2]);
+                    if (page_next[b] < 0 && lane == 0) raise_error(c.err, kErrBounds);
+                }
+            }
+        };
+        // unit u's blocks (pages in page_next) into their stage
+        auto fetch = [&](int u) {
+            if (u < u1) {
+                const int stage = (u - u0) % Cfg::STAGES;
+                const uint32_t dst = ring + stage * Cfg::STAGE;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * b), pg = page_next[b];
+                    FewBlock& block = s_block[warp][stage][b];
+                    if (lane == 0) block.page = pg;
+                    if (pg < 0) continue;
+                    const size_t at = (size_t)(unsigned)pg * page_codes + (unsigned)(slot * hd) + my_at;
+                    if (lane < 2) {
+                        const size_t sa = (size_t)(unsigned)pg * page_scales + (slot >> 4);
+                        cp_async4(smem_addr(lane ? &block.vs : &block.ks), (lane ? vsbase : ksbase) + sa);
+                    }
+                    if (copies) {
+                        const int8_t *kp = c.k + at, *vp = c.v + at;
+#pragma unroll
+                        for (int r = 0; r < 16; r += ROWS) {
+                            cp_async16(dst + (16 * b + r) * DP + (key_to ^ 16 * few_key_swizzle<DP>(r)), kp + r * hd);
+                            cp_async16(dst + (Cfg::TB + 16 * b + r) * DP + (value_to ^ 16 * few_value_swizzle<DP>(r)), vp + r * hd);
+                        }
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+        find(u0);
+#pragma unroll
+        for (int i = 0; i < Cfg::STAGES - 1; i++) {
+            fetch(u0 + i);
+            find(u0 + i + 1);
+        }
+        // ---- the columns' queries and what they see ----
+        // A warp turns a column at a time into its digits; everyone then takes
+        // its A fragments (rows g: column g) from shared memory. The integer
+        // product's k index runs over 16 t + 4 q4 + byte of a 32-dim step:
+        // words 0, 1 and 2, 3 of the 16 dims a lane's key pieces hold.
+        for (int k = warp; k < COLS; k += kFewWarps) {
+            float amax = 0.0f, x[(DP + 127) / 128][4];
+            bool wild = false;  // infinities and NaN have no digits
+            const size_t at = k < cols ? (size_t)(seg.row + k / heads) * a.q_stride + (size_t)(h0 + k % heads) * hd : 0;
+#pragma unroll
+            for (int v = 0; v < (DP + 127) / 128; v++) {
+                const int d = 128 * v + 4 * lane;
+                x[v][0] = x[v][1] = x[v][2] = x[v][3] = 0.0f;
+                if (k < cols && d < hd) load4<DT>(a.q, at + d, x[v]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    amax = fmaxf(amax, fabsf(x[v][i]));
+                    wild |= !(fabsf(x[v][i]) <= 0x1.fffffep127f);
+                }
+            }
+            const float up = kv_query_scale(warp_max_abs(amax));
+            wild = __any_sync(0xffffffffu, wild);
+#pragma unroll
+            for (int v = 0; v < (DP + 127) / 128; v++) {
+                uint32_t d[3];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[v][i] *= up;
+                kv_query_digits(x[v], d);
+                if (128 * v + 4 * lane < DP) {
+#pragma unroll
+                    for (int z = 0; z < 3; z++) *reinterpret_cast<uint32_t*>(&s_q[z][k][128 * v + 4 * lane]) = d[z];
+                }
+            }
+            if (lane == 0) {
+                s_f[k] = wild ? __int_as_float(0x7fc00000) : a.scale * kLog2e / up;  // NaN: so are the column's scores
+                int end = 0;
+                if (k < cols) {
+                    const int p = a.positions[seg.row + k / heads];
+                    end = p >= 0 && p < seg.hi ? p + 1 : 0;
+                }
+                s_end[k] = end;
+            }
+        }
+        __syncthreads();
         uint32_t qf[3][NT][KC * 2][2];
         float qs[NT];
         int end[NT], begin[NT];
         int all_lo = 0, all_hi = INT_MAX;  // tokens every column sees
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int col = nt * 8 + g;
-            const bool in = col < cols;
-            const size_t at = in ? (size_t)(seg.row + col / heads) * a.q_stride + (size_t)(h0 + col % heads) * hd : 0;
-            float x[KC][4][4];
-            float amax = 0.0f;
+            const int k = nt * 8 + g;
 #pragma unroll
-            for (int p = 0; p < KC; p++) {
-                const int d = 64 * p + 16 * q4;
+            for (int z = 0; z < 3; z++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    x[p][w][0] = x[p][w][1] = x[p][w][2] = x[p][w][3] = 0.0f;
-                    if (in && d < hd) load4<DT>(a.q, at + d + 4 * w, x[p][w]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(x[p][w][i]));
+                for (int p = 0; p < KC; p++) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(&s_q[z][k][64 * p + 16 * q4]);
+                    qf[z][nt][2 * p][0] = x.x;
+                    qf[z][nt][2 * p][1] = x.y;
+                    qf[z][nt][2 * p + 1][0] = x.z;
+                    qf[z][nt][2 * p + 1][1] = x.w;
                 }
-            }
-            bool wild = false;  // infinities and NaN have no digits
-#pragma unroll
-            for (int p = 0; p < KC; p++)
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) wild |= !(fabsf(x[p][w][i]) <= 0x1.fffffep127f);
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const unsigned wilds = __ballot_sync(0xffffffffu, wild);
-            float up = kv_query_scale(amax);
-#pragma unroll
-            for (int p = 0; p < KC; p++)
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    uint32_t d[3];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[p][w][i] *= up;
-                    kv_query_digits(x[p][w], d);
-#pragma unroll
-                    for (int z = 0; z < 3; z++) qf[z][nt][2 * p + (w >> 1)][w & 1] = d[z];
-                }
-            if (wilds >> (4 * g) & 15u) up = __int_as_float(0x7fc00000);  // the column's scores become NaN
-            qs[nt] = a.scale * kLog2e / up;
-            end[nt] = begin[nt] = 0;
-            if (in) {
-                const int p = a.positions[seg.row + col / heads];
-                end[nt] = p >= 0 && p < seg.hi ? p + 1 : 0;
-                begin[nt] = a.window > 0 ? max(0, end[nt] - a.window) : 0;
+            qs[nt] = s_f[k];
+            end[nt] = s_end[k];
+            begin[nt] = a.window > 0 ? max(0, end[nt] - a.window) : 0;
+            if (k < cols) {
                 all_hi = min(all_hi, end[nt]);
                 all_lo = max(all_lo, begin[nt]);
             }
@@ -435,83 +642,14 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
 #pragma unroll
             for (int i = 0; i < MT; i++) acc[i][nt][0] = acc[i][nt][1] = acc[i][nt][2] = acc[i][nt][3] = 0.0f;
         }
-        const int32_t* row = c.table + (size_t)min(seg.seq, c.n_seqs - 1) * c.max_pages;
-        // a page's codes and scales (at most 2^26 bytes), and this lane's place in a block
-        const unsigned page_codes = (unsigned)(c.nkv * hd) << c.page_log2, page_scales = (unsigned)c.nkv << c.page_log2 >> 4;
-        const int8_t* kbase = c.k + ((size_t)head << c.page_log2) * hd + (unsigned)(g * hd) + (HD ? 16 * q4 : 0);
-        const int8_t* vbase = c.v + ((size_t)head << c.page_log2) * hd + (unsigned)(2 * q4 * hd) + (HD ? 4 * VW * g : 0);
-        const float* ksbase = c.ks + ((size_t)head << c.page_log2 >> 4);
-        const float* vsbase = c.vs + ((size_t)head << c.page_log2 >> 4);
-
-        // ---- tokens ----
-        uint4 kr[NB][2][KC];          // tokens g and g + 8 of each block
-        uint32_t vr[NB][4][VW];       // tokens 2 q4, + 1, + 8, + 9
-        float ks[NB], vs[NB], ks_next[NB], vs_next[NB];
-        int page[NB], page_next[NB];
-        // page of each block of unit u, -1: nothing of it is seen, or it is missing
-        auto find = [&](int u, int (&pg)[NB]) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const int t = u * CH + warp * Cfg::TB + 16 * b;
-                pg[b] = -1;
-                if (u < u1 && t < seg.hi && t + 16 > seg.lo) {
-                    pg[b] = c.checked(row[t >> c.page_log2]);
-                    if (pg[b] < 0 && lane == 0) raise_error(c.err, kErrBounds);
-                }
-            }
-        };
-        auto load_k = [&](int u, const int (&pg)[NB], float (&fk)[NB], float (&fv)[NB]) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * b);
-                const unsigned pn = (unsigned)max(pg[b], 0);
-                fk[b] = ksbase[(size_t)pn * page_scales + (slot >> 4)];
-                fv[b] = vsbase[(size_t)pn * page_scales + (slot >> 4)];
-                if (pg[b] < 0) fk[b] = fv[b] = 0.0f;
-                const int8_t* src = kbase + (size_t)pn * page_codes + (unsigned)(slot * hd);
-#pragma unroll
-                for (int p = 0; p < KC; p++) {
-                    const int d = HD ? 64 * p : min(64 * p + 16 * q4, hd - 16);
-                    kr[b][0][p] = load_stream16(src + d);
-                    kr[b][1][p] = load_stream16(src + 8 * hd + d);
-                }
-            }
-        };
-        auto load_v = [&](int u, const int (&pg)[NB]) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * b);
-                const int8_t* src = vbase + (size_t)(unsigned)max(pg[b], 0) * page_codes + (unsigned)(slot * hd);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int8_t* p = src + ((j & 1) + 8 * (j >> 1)) * hd;
-                    if (VW == 2) {
-                        const uint2 v = load_stream8(p);
-                        vr[b][j][0] = v.x;
-                        vr[b][j][1] = v.y;
-                    } else {
-#pragma unroll
-                        for (int w = 0; w + 4 <= VW; w += 4) {
-                            const uint4 v = load_stream16(p + (HD ? 4 * w : min(4 * VW * g + 4 * w, hd - 16)));
-                            vr[b][j][w] = v.x;
-                            vr[b][j][w + 1] = v.y;
-                            vr[b][j][w + 2] = v.z;
-                            vr[b][j][w + 3] = v.w;
-                        }
-                    }
-                }
-            }
-        };
-        find(u0, page);
-        load_k(u0, page, ks, vs);
-        load_v(u0, page);
-        find(u0 + 1, page_next);
+        int page[NB];
+        float ks[NB], vs[NB];
         // One step over the warp's tokens of unit u; WHOLE: every column sees
         // all of them and every page is there.
         auto step = [&](int u, auto whole) {
             constexpr bool WHOLE = decltype(whole)::value;
-            const int t0 = u * CH + warp * Cfg::TB;
-            const bool more = u + 1 < u1;
+            const int t0 = u * CH + warp * Cfg::TB, stage = (u - u0) % Cfg::STAGES;
+            const uint32_t keys = ring + stage * Cfg::STAGE, vals = keys + Cfg::TB * DP + value_at;
             // q . kc, integers of at most 2^45, rounded to f32; [token half][token]
             float s[NB][NT][4];
 #pragma unroll
@@ -520,27 +658,25 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 for (int j = 0; j < 2; j++) {
                     int z[NT][4], lo[(NT + 1) / 2][4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0;
-#pragma unroll
-                    for (int i = 0; i < (NT + 1) / 2; i++) lo[i][0] = lo[i][1] = lo[i][2] = lo[i][3] = 0;
-#pragma unroll
                     for (int p = 0; p < KC; p++) {
-                        const uint4 x = kr[b][j][p];
+                        const uint4 x = load_shared16(keys + (16 * b + 8 * j) * DP + 128 * (p / 2) + key_at[p & 1]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            mma_s8(z[nt], qf[0][nt][2 * p][0], qf[1][nt][2 * p][0], qf[0][nt][2 * p][1], qf[1][nt][2 * p][1],
-                                   x.x, x.y);
-                            mma_s8(z[nt], qf[0][nt][2 * p + 1][0], qf[1][nt][2 * p + 1][0], qf[0][nt][2 * p + 1][1],
-                                   qf[1][nt][2 * p + 1][1], x.z, x.w);
-                        }
+                        for (int h = 0; h < 2; h++) {  // the two 32-dim steps of a piece
+                            const uint32_t b0 = h ? x.z : x.x, b1 = h ? x.w : x.y;
 #pragma unroll
-                        for (int i = 0; i < (NT + 1) / 2; i++) {  // the lowest digits of two sets of columns
-                            constexpr int last = NT - 1;
-                            const int n0 = 2 * i, n1 = NT == 1 ? 0 : (2 * i + 1 < last ? 2 * i + 1 : last);
-                            mma_s8(lo[i], qf[2][n0][2 * p][0], qf[2][n1][2 * p][0], qf[2][n0][2 * p][1], qf[2][n1][2 * p][1],
-                                   x.x, x.y);
-                            mma_s8(lo[i], qf[2][n0][2 * p + 1][0], qf[2][n1][2 * p + 1][0], qf[2][n0][2 * p + 1][1],
-                                   qf[2][n1][2 * p + 1][1], x.z, x.w);
+                            for (int nt = 0; nt < NT; nt++) {
+                                const auto& hi = qf[0][nt][2 * p + h];
+                                const auto& mid = qf[1][nt][2 * p + h];
+                                if (p + h == 0) mma_s8<true>(z[nt], hi[0], mid[0], hi[1], mid[1], b0, b1);
+                                else mma_s8<false>(z[nt], hi[0], mid[0], hi[1], mid[1], b0, b1);
+                            }
+#pragma unroll
+                            for (int i = 0; i < (NT + 1) / 2; i++) {  // the lowest digits of two sets of columns
+                                const auto& l0 = qf[2][2 * i][2 * p + h];
+                                const auto& l1 = qf[2][2 * i + 1 < NT ? 2 * i + 1 : 2 * i][2 * p + h];
+                                if (p + h == 0) mma_s8<true>(lo[i], l0[0], l1[0], l0[1], l1[1], b0, b1);
+                                else mma_s8<false>(lo[i], l0[0], l1[0], l0[1], l1[1], b0, b1);
+                            }
                         }
                     }
 #pragma unroll
@@ -550,7 +686,6 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                             s[b][nt][2 * j + e] = fmaf((float)z[nt][e], 65536.0f,
                                                        (float)(z[nt][2 + e] * 256 + lo[nt / 2][2 * (nt & 1) + e]));
                 }
-            if (more) load_k(u + 1, page_next, ks_next, vs_next);
             // score = s f in units of log 2
             float f[NB][NT], top[NT];
             bool hidden[NB][NT][4], raise = false;
@@ -601,6 +736,25 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const float fv = vs[b] * vinv;
+                uint32_t vr[4][VW];  // tokens 2 q4, + 1, + 8, + 9
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t src = vals + (16 * b + (j & 1) + 8 * (j >> 1)) * DP;
+                    if (VW == 2) {
+                        const uint2 v = load_shared8(src);
+                        vr[j][0] = v.x;
+                        vr[j][1] = v.y;
+                    } else {
+#pragma unroll
+                        for (int w = 0; w + 4 <= VW; w += 4) {
+                            const uint4 v = load_shared16(src + 4 * w);
+                            vr[j][w] = v.x;
+                            vr[j][w + 1] = v.y;
+                            vr[j][w + 2] = v.z;
+                            vr[j][w + 3] = v.w;
+                        }
+                    }
+                }
                 uint32_t pf[SPLIT][NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -625,8 +779,8 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 }
 #pragma unroll
                 for (int i = 0; i < VW; i++) {
-                    const uint32_t lo01 = __byte_perm(vr[b][0][i], vr[b][1][i], 0x5410), hi01 = __byte_perm(vr[b][0][i], vr[b][1][i], 0x7632);
-                    const uint32_t lo23 = __byte_perm(vr[b][2][i], vr[b][3][i], 0x5410), hi23 = __byte_perm(vr[b][2][i], vr[b][3][i], 0x7632);
+                    const uint32_t lo01 = __byte_perm(vr[0][i], vr[1][i], 0x5410), hi01 = __byte_perm(vr[0][i], vr[1][i], 0x7632);
+                    const uint32_t lo23 = __byte_perm(vr[2][i], vr[3][i], 0x5410), hi23 = __byte_perm(vr[2][i], vr[3][i], 0x7632);
                     const uint32_t a0 = codes_even(lo01), a1 = codes_odd(lo01), a2 = codes_even(lo23), a3 = codes_odd(lo23);
                     const uint32_t b0 = codes_even(hi01), b1 = codes_odd(hi01), b2 = codes_even(hi23), b3 = codes_odd(hi23);
 #pragma unroll
@@ -638,25 +792,27 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                         }
                 }
             }
-            if (more) {
-                load_v(u + 1, page_next);
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    page[b] = page_next[b];
-                    ks[b] = ks_next[b];
-                    vs[b] = vs_next[b];
-                }
-                find(u + 2, page_next);
-            }
         };
         for (int u = u0; u < u1; u++) {
-            const int t0 = u * CH + warp * Cfg::TB;
+            fetch(u + Cfg::STAGES - 1);
+            find(u + Cfg::STAGES);
+            cp_async_wait<Cfg::STAGES - 1>();
+            __syncwarp();
+            const int t0 = u * CH + warp * Cfg::TB, stage = (u - u0) % Cfg::STAGES;
             bool whole = t0 >= all_lo && t0 + Cfg::TB <= all_hi;
 #pragma unroll
-            for (int b = 0; b < NB; b++) whole = whole && page[b] >= 0;
+            for (int b = 0; b < NB; b++) {
+                const FewBlock block = s_block[warp][stage][b];
+                page[b] = block.page;
+                ks[b] = page[b] < 0 ? 0.0f : block.ks;
+                vs[b] = page[b] < 0 ? 0.0f : block.vs;
+                whole = whole && page[b] >= 0;
+            }
             if (whole) step(u, std::true_type{});
             else step(u, std::false_type{});
+            __syncwarp();
         }
+        cp_async_wait<0>();
 
         // ---- the four warps' parts joined ----
         const float unscale = vtop / kWeightTop;
@@ -696,73 +852,26 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
             s_inv[tid] = sum;
         }
         __syncthreads();
-        const bool split = tile0 < walk.begin || tile1 > walk.end;
+        const bool split = first < walk.begin || tile1 > walk.end;
         const int quads = hd / 4;
-        int c0 = 0, c1 = 0;
-        if (split) {
-            // this CTA's part to the workspace; the last to arrive joins them
-            c0 = walk.owner(tile0);
-            c1 = walk.owner(tile1 - 1);
-            float* part = a.parts + ((size_t)2 * blockIdx.x + (tile0 >= walk.begin)) * a.part_floats;
-            for (int i = tid; i < cols * quads; i += kFewThreads) {
-                const int k = i / quads, d = 4 * (i - k * quads);
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float* part = a.parts + ((size_t)2 * blockIdx.x + (first >= walk.begin)) * a.part_floats;
+        for (int i = tid; i < cols * quads; i += kFewThreads) {
+            const int k = i / quads, d = 4 * (i - k * quads);
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 0; w < kFewWarps; w++) {
-                    const float4 y = *reinterpret_cast<const float4*>(s_acc + ((size_t)w * COLS + k) * DP + d);
-                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-                }
-                __stcg(reinterpret_cast<float4*>(part + 2 * COLS + (size_t)k * hd + d), x);
+            for (int w = 0; w < kFewWarps; w++) {
+                const float4 y = *reinterpret_cast<const float4*>(s_acc + ((size_t)w * COLS + k) * DP + d);
+                x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
             }
-            if (tid < cols) {
-                __stcg(part + tid, s_f[tid]);
-                __stcg(part + COLS + tid, s_inv[tid]);
-            }
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const unsigned before = atomicAdd(&a.arrived[c0], 1u);
-                s_last = before == (unsigned)(c1 - c0);
-                if (s_last) a.arrived[c0] = 0;
-            }
-            __syncthreads();
-            if (s_last) __threadfence();
+            if (split) *reinterpret_cast<float4*>(part + 2 * COLS + 4 * i) = make_float4(x[0], x[1], x[2], x[3]);
+            else kv_finish<DT>(a, seg.row + k / heads, h0 + k % heads, hd, d, x, s_f[k], s_inv[k]);
         }
-        if (!split || s_last) {
-            for (int i = tid; i < cols * quads; i += kFewThreads) {
-                const int k = i / quads, d = 4 * (i - k * quads);
-                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum, top;
-                if (!split) {
-                    sum = s_inv[k];
-                    top = s_f[k];
-#pragma unroll
-                    for (int w = 0; w < kFewWarps; w++) {
-                        const float4 y = *reinterpret_cast<const float4*>(s_acc + ((size_t)w * COLS + k) * DP + d);
-                        x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
-                    }
-                } else {
-                    top = none;
-                    for (int r = c0; r <= c1; r++)
-                        top = fmaxf(top, __ldcg(a.parts + ((size_t)2 * r + (r == c0)) * a.part_floats + k));
-                    sum = 0.0f;
-                    for (int r = c0; r <= c1; r++) {
-                        const float* part = a.parts + ((size_t)2 * r + (r == c0)) * a.part_floats;
-                        const float mr = __ldcg(part + k), f = mr == none ? 1.0f : exp2_fast(mr - top);
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part + 2 * COLS + (size_t)k * hd + d));
-                        sum += f * __ldcg(part + COLS + k);
-                        x[0] = fmaf(f, y.x, x[0]); x[1] = fmaf(f, y.y, x[1]);
-                        x[2] = fmaf(f, y.z, x[2]); x[3] = fmaf(f, y.w, x[3]);
-                    }
-                }
-                const bool empty = top == none && sum == 0.0f;  // nothing seen
-                const int r = seg.row + k / heads, h = h0 + k % heads;
-                const float inv = empty ? 0.0f : __fdiv_rn(1.0f, sum);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = empty ? 0.0f : x[e] * inv;
-                store4<DT>(a.out, (size_t)r * a.out_stride + (size_t)h * hd + d, x);
-                if (d == 0 && a.lse) a.lse[(size_t)r * a.nh + h] = empty ? none : (top + log2f(sum)) * kLn2;
-            }
+        if (split && tid < cols) {
+            part[tid] = s_f[tid];
+            part[COLS + tid] = s_inv[tid];
         }
+        if (split && first >= walk.begin && tid == 0)
+            a.splits[blockIdx.x] = {(int)walk.owner(tile1 - 1) - (int)blockIdx.x + 1, cols, heads, seg.row, h0};
         __syncthreads();
         unit = min(tile1, walk.end);
     }

@@ -37,8 +37,8 @@ struct ServingWs {
     static constexpr size_t kPairsOff = 256;
     static constexpr size_t kPairsBytes = (size_t)kMaxKvPages / 2 * 4;
     static constexpr size_t kPartsOff = kPairsOff + 2 * kPairsBytes;
-    static constexpr size_t kArrivedOff = kPartsOff + (size_t)kVerifyParts * sizeof(VerifyPart);
-    static constexpr size_t kAttnOff = kArrivedOff + kAttnMaxGrid * 4;
+    static constexpr size_t kSplitsOff = kPartsOff + (size_t)kVerifyParts * sizeof(VerifyPart);
+    static constexpr size_t kAttnOff = kSplitsOff + kAttnMaxGrid * sizeof(KvSplit);
     static constexpr size_t kTotal = kAttnOff + kAttnPartBytes;
     uint8_t* base;
     PagePairs pairs() const {
@@ -46,7 +46,7 @@ struct ServingWs {
                 reinterpret_cast<int32_t*>(base + kPairsOff + kPairsBytes)};
     }
     VerifyPart* parts() const { return reinterpret_cast<VerifyPart*>(base + kPartsOff); }
-    unsigned* arrived() const { return reinterpret_cast<unsigned*>(base + kArrivedOff); }
+    KvSplit* splits() const { return reinterpret_cast<KvSplit*>(base + kSplitsOff); }
     float* attn_parts() const { return reinterpret_cast<float*>(base + kAttnOff); }
 };
 
@@ -140,9 +140,48 @@ hale_status check_layer_rows(hale_ctx* ctx, const hale_kv8* kv, const char* what
 // CTAs of an attention launch: what the GPU holds at once, no more than there
 // can be units of CH tokens, and no more than the workspace has parts for.
 unsigned attn_grid(const hale_ctx* ctx, const KvArgs& c, const KvAttn& a, int per_sm, int chunk) {
-    const uint64_t units = (uint64_t)a.n * c.nkv * a.subs * (((uint64_t)c.capacity() + chunk - 1) / chunk);
+    const uint64_t units = (uint64_t)a.n * c.nkv * a.subs * ((uint64_t)c.capacity() / chunk + 1 + kTileCost);
     const uint64_t parts = kAttnPartBytes / 8 / a.part_floats;
     return (unsigned)std::min<uint64_t>({(uint64_t)ctx->sm_count * per_sm, units, parts, (uint64_t)kAttnMaxGrid});
+}
+
+// Rows of one launch: units are counted in 32 bits.
+uint32_t attn_rows(const KvArgs& c, const KvAttn& a, int chunk) {
+    const uint64_t row = (uint64_t)c.nkv * a.subs * ((uint64_t)c.capacity() / chunk + 1 + kTileCost);
+    const uint64_t rows = std::max<uint64_t>(1, 0x7fffffffull / row) / a.rows * a.rows;
+    return (uint32_t)std::min<uint64_t>((uint64_t)a.n, std::max<uint64_t>(rows, (uint64_t)a.rows));
+}
+
+// Rows i .. i + n - 1 of a call.
+template <int DT>
+KvAttn attn_part(const KvAttn& a, uint32_t i, uint32_t n) {
+    constexpr size_t el = DT == 0 ? 4 : 2;
+    KvAttn b = a;
+    b.q = static_cast<const char*>(a.q) + i * a.q_stride * el;
+    b.out = static_cast<char*>(a.out) + i * a.out_stride * el;
+    b.lse = a.lse ? a.lse + (size_t)i * a.nh : nullptr;
+    b.seqs = a.seqs ? a.seqs + i : nullptr;
+    b.positions = a.positions + i;
+    b.n = (int)n;
+    return b;
+}
+
+// The joining launch may begin while the CTAs before it finish (it waits for
+// them itself).
+template <int DT>
+hale_status attn_join(hale_ctx* ctx, const KvAttn& a, int hd, int cols, unsigned grid, cudaStream_t st) {
+    if (grid == 1) return HALE_OK;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kv_join_kernel<DT>, a, hd, cols));
+    return check_launch(ctx, "kv_join");
 }
 
 template <int DT, int DP, int HD, int NT>
@@ -152,11 +191,17 @@ hale_status attn_few(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cud
     a.subs = (a.group + a.heads - 1) / a.heads;
     a.rows = (int)std::max<uint32_t>(1u, std::min<uint32_t>(run, (uint32_t)(cols / a.heads)));
     a.part_floats = cols * (2 + c.hd);
-    const size_t smem = (size_t)kFewWarps * cols * DP * 4;
+    const size_t smem = std::max((size_t)kFewWarps * cols * DP * 4, (size_t)kFewWarps * FewCfg<DP>::RING);
     CUDA_TRY(ctx, allow_smem(kv_attn_few_kernel<DT, DP, HD, NT>, smem));
-    const unsigned grid = attn_grid(ctx, c, a, DP <= 128 && NT == 1 ? 3 : 2, FewCfg<DP>::CH);
-    kv_attn_few_kernel<DT, DP, HD, NT><<<grid, kFewThreads, smem, st>>>(c, a);
-    return check_launch(ctx, "kv_attn_few");
+    const uint32_t step = attn_rows(c, a, FewCfg<DP>::CH), n = (uint32_t)a.n;
+    for (uint32_t i = 0; i < n; i += step) {
+        const KvAttn b = attn_part<DT>(a, i, std::min(step, n - i));
+        const unsigned grid = attn_grid(ctx, c, b, DP <= 128 && NT == 1 ? 3 : 2, FewCfg<DP>::CH);
+        kv_attn_few_kernel<DT, DP, HD, NT><<<grid, kFewThreads, smem, st>>>(c, b);
+        if (hale_status r = check_launch(ctx, "kv_attn_few")) return r;
+        if (hale_status r = attn_join<DT>(ctx, b, c.hd, cols, grid, st)) return r;
+    }
+    return HALE_OK;
 }
 
 template <int DT>
@@ -287,7 +332,7 @@ extern "C" hale_status hale_kv8_attention(hale_ctx* ctx, const hale_kv8* kv, uin
     ServingWs ws;
     if ((r = serving_ws(ctx, stream, &ws))) return r;
     a.parts = ws.attn_parts();
-    a.arrived = ws.arrived();
+    a.splits = ws.splits();
     ProfScope ps(ctx, "kv8_attention", S(stream));
     switch (dtype) {
     case HALE_F32: return attn_go<0>(ctx, c, a, run, S(stream));

@@ -495,7 +495,6 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         const int h0 = head * a.group + sub * a.heads;  // the tile's first query head
 
         // ---- the first tokens are under way while the queries are prepared ----
-        const int32_t* row = c.table + (size_t)min(seg.seq, c.n_seqs - 1) * c.max_pages;
         // a page's codes (at most 2^26 bytes) and scales
         const unsigned page_codes = (unsigned)(c.nkv * hd) << c.page_log2, page_scales = (unsigned)c.nkv << c.page_log2 >> 4;
         // this lane's pieces: 32 / PIECES rows apart
@@ -514,53 +513,58 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         const float* ksbase = c.ks + ((size_t)head << c.page_log2 >> 4);
         const float* vsbase = c.vs + ((size_t)head << c.page_log2 >> 4);
 
-        // page of each block of unit u, -1: nothing of it is seen, or it is missing
-        int page_next[NB];
+        // Pages of the warp's blocks: lane i holds that of block i of 32, a page
+        // piece (PB blocks that lie in one page) an entry; the next 32 are
+        // under way. -1: nothing of it is seen, or it is missing.
+        constexpr int PB = HD ? NB : 1, PER = NB / PB;  // (a page of 16 tokens takes the kernels of any head size)
+        const int32_t* row = c.table + (size_t)min(seg.seq, c.n_seqs - 1) * c.max_pages;
         auto find = [&](int u) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const int t = u * CH + warp * Cfg::TB + 16 * b;
-                page_next[b] = -1;
-                if (u < u1 && t < seg.hi && t + 16 > seg.lo) {
-                    page_next[b] = c.checked(row[t >> c.page_log2]);
-                    if (page_next[b] < 0 && lane == 0) raise_error(c.err, kErrBounds);
-                }
+            const int t = (u + lane / PER) * CH + warp * Cfg::TB + 16 * PB * (lane % PER);
+            int pg = -1;
+            if (u + lane / PER < u1 && t < seg.hi && t + 16 * PB > seg.lo) {
+                pg = c.checked(row[t >> c.page_log2]);
+                if (pg < 0) raise_error(c.err, kErrBounds);
             }
+            return pg;
         };
-        // unit u's blocks (pages in page_next) into their stage
+        int pages = find(u0), pages_next = find(u0 + 32 / PER), pages_from = u0;
+        // unit u's codes and scales into their stage
         auto fetch = [&](int u) {
             if (u < u1) {
+                if (u - pages_from == 32 / PER) {
+                    pages = pages_next;
+                    pages_from = u;
+                    pages_next = find(u + 32 / PER);
+                }
                 const int stage = (u - u0) % Cfg::STAGES;
                 const uint32_t dst = ring + stage * Cfg::STAGE;
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * b), pg = page_next[b];
-                    FewBlock& block = s_block[warp][stage][b];
-                    if (lane == 0) block.page = pg;
+                for (int e = 0; e < PER; e++) {
+                    const int pg = __shfl_sync(0xffffffffu, pages, (u - pages_from) * PER + e);
+                    const int slot = c.slot(u * CH + warp * Cfg::TB + 16 * PB * e);
+                    FewBlock* block = s_block[warp][stage] + PB * e;
+                    if (lane < PB) block[lane].page = pg;
                     if (pg < 0) continue;
-                    const size_t at = (size_t)(unsigned)pg * page_codes + (unsigned)(slot * hd) + my_at;
-                    if (lane < 2) {
-                        const size_t sa = (size_t)(unsigned)pg * page_scales + (slot >> 4);
-                        cp_async4(smem_addr(lane ? &block.vs : &block.ks), (lane ? vsbase : ksbase) + sa);
+                    if (lane < 2 * PB) {
+                        const size_t sa = (size_t)(unsigned)pg * page_scales + (slot >> 4) + (lane >> 1);
+                        cp_async4(smem_addr(lane & 1 ? &block[lane >> 1].vs : &block[lane >> 1].ks), (lane & 1 ? vsbase : ksbase) + sa);
                     }
                     if (copies) {
+                        const size_t at = (size_t)(unsigned)pg * page_codes + (unsigned)(slot * hd) + my_at;
                         const int8_t *kp = c.k + at, *vp = c.v + at;
 #pragma unroll
-                        for (int r = 0; r < 16; r += ROWS) {
-                            cp_async16(dst + (16 * b + r) * DP + (key_to ^ 16 * few_key_swizzle<DP>(r)), kp + r * hd);
-                            cp_async16(dst + (Cfg::TB + 16 * b + r) * DP + (value_to ^ 16 * few_value_swizzle<DP>(r)), vp + r * hd);
+                        for (int r = 0; r < 16 * PB; r += ROWS) {
+                            cp_async16(dst + (16 * PB * e + r) * DP + (key_to ^ 16 * few_key_swizzle<DP>(r)), kp + r * hd);
+                            cp_async16(dst + (Cfg::TB + 16 * PB * e + r) * DP + (value_to ^ 16 * few_value_swizzle<DP>(r)),
+                                       vp + r * hd);
                         }
                     }
                 }
             }
             cp_async_commit();
         };
-        find(u0);
 #pragma unroll
-        for (int i = 0; i < Cfg::STAGES - 1; i++) {
-            fetch(u0 + i);
-            find(u0 + i + 1);
-        }
+        for (int i = 0; i < Cfg::STAGES - 1; i++) fetch(u0 + i);
         // ---- the columns' queries and what they see ----
         // A warp turns a column at a time into its digits; everyone then takes
         // its A fragments (rows g: column g) from shared memory. The integer
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
             }
         }
         __syncthreads();
-        uint32_t qf[3][NT][KC * 2][2];
+        uint32_t qf[2][NT][KC * 2][2], qlo[(NT + 1) / 2][KC * 2][4];
         float qs[NT];
         int end[NT], begin[NT];
         int all_lo = 0, all_hi = INT_MAX;  // tokens every column sees
@@ -613,7 +617,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         for (int nt = 0; nt < NT; nt++) {
             const int k = nt * 8 + g;
 #pragma unroll
-            for (int z = 0; z < 3; z++)
+            for (int z = 0; z < 2; z++)
 #pragma unroll
                 for (int p = 0; p < KC; p++) {
                     const uint4 x = *reinterpret_cast<const uint4*>(&s_q[z][k][64 * p + 16 * q4]);
@@ -630,6 +634,21 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                 all_lo = max(all_lo, begin[nt]);
             }
         }
+        // the lowest digits of two sets of columns (of one: twice) as whole
+        // operands; read by loads of their own, so that the second copy is no
+        // register moved before every product
+#pragma unroll
+        for (int i = 0; i < (NT + 1) / 2; i++)
+#pragma unroll
+            for (int p = 0; p < KC; p++) {
+                const uint32_t at = smem_addr(&s_q[2][16 * i + g][64 * p + 16 * q4]);
+                const uint4 x = load_shared16(at), y = load_shared16(2 * i + 1 < NT ? at + 8 * (DP + 16) : at);
+                const uint32_t quads[2][4] = {{x.x, y.x, x.y, y.y}, {x.z, y.z, x.w, y.w}};
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) qlo[i][2 * p + h][e] = quads[h][e];
+            }
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
 
@@ -671,11 +690,10 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
                                 else mma_s8<false>(z[nt], hi[0], mid[0], hi[1], mid[1], b0, b1);
                             }
 #pragma unroll
-                            for (int i = 0; i < (NT + 1) / 2; i++) {  // the lowest digits of two sets of columns
-                                const auto& l0 = qf[2][2 * i][2 * p + h];
-                                const auto& l1 = qf[2][2 * i + 1 < NT ? 2 * i + 1 : 2 * i][2 * p + h];
-                                if (p + h == 0) mma_s8<true>(lo[i], l0[0], l1[0], l0[1], l1[1], b0, b1);
-                                else mma_s8<false>(lo[i], l0[0], l1[0], l0[1], l1[1], b0, b1);
+                            for (int i = 0; i < (NT + 1) / 2; i++) {
+                                const auto& q = qlo[i][2 * p + h];
+                                if (p + h == 0) mma_s8<true>(lo[i], q[0], q[1], q[2], q[3], b0, b1);
+                                else mma_s8<false>(lo[i], q[0], q[1], q[2], q[3], b0, b1);
                             }
                         }
                     }
@@ -795,7 +813,6 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         };
         for (int u = u0; u < u1; u++) {
             fetch(u + Cfg::STAGES - 1);
-            find(u + Cfg::STAGES);
             cp_async_wait<Cfg::STAGES - 1>();
             __syncwarp();
             const int t0 = u * CH + warp * Cfg::TB, stage = (u - u0) % Cfg::STAGES;
@@ -804,9 +821,20 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
             for (int b = 0; b < NB; b++) {
                 const FewBlock block = s_block[warp][stage][b];
                 page[b] = block.page;
-                ks[b] = page[b] < 0 ? 0.0f : block.ks;
-                vs[b] = page[b] < 0 ? 0.0f : block.vs;
+                ks[b] = block.ks;
+                vs[b] = block.vs;
                 whole = whole && page[b] >= 0;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    // a block no row sees a token of: its scales may be anything
+                    const int t = t0 + 16 * b;
+                    if (page[b] < 0 || t >= seg.hi || t + 16 <= seg.lo) {
+                        page[b] = -1;
+                        ks[b] = vs[b] = 0.0f;
+                    }
+                }
             }
             if (whole) step(u, std::true_type{});
             else step(u, std::false_type{});

@@ -207,16 +207,18 @@ hale_status attn_few(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cud
 template <int DT>
 hale_status attn_go(hale_ctx* ctx, const KvArgs& c, const KvAttn& a, uint32_t run, cudaStream_t st) {
     const uint64_t cols = (uint64_t)std::min<uint32_t>(run, (uint32_t)a.n) * a.group;
+    // the kernels of a known head size take two blocks of 16 tokens from one page
+    const int hd = c.page_log2 == 4 ? 0 : c.hd;
     if (cols <= 8) {
-        switch (c.hd) {
+        switch (hd) {
         case 64: return attn_few<DT, 64, 64, 1>(ctx, c, a, run, st);
         case 128: return attn_few<DT, 128, 128, 1>(ctx, c, a, run, st);
         case 256: return attn_few<DT, 256, 256, 1>(ctx, c, a, run, st);
-        default: return c.hd < 128 ? attn_few<DT, 128, 0, 1>(ctx, c, a, run, st) : attn_few<DT, 256, 0, 1>(ctx, c, a, run, st);
+        default: return c.hd <= 128 ? attn_few<DT, 128, 0, 1>(ctx, c, a, run, st) : attn_few<DT, 256, 0, 1>(ctx, c, a, run, st);
         }
     }
     if (cols <= 16 && c.hd <= 128) {
-        switch (c.hd) {
+        switch (hd) {
         case 64: return attn_few<DT, 64, 64, 2>(ctx, c, a, run, st);
         case 128: return attn_few<DT, 128, 128, 2>(ctx, c, a, run, st);
         default: return attn_few<DT, 128, 0, 2>(ctx, c, a, run, st);

@@ -62,15 +62,15 @@ constexpr int kAttnMaxGrid = 1024;
 struct KvSegment {
     int row, rows, seq;
     int lo, hi;      // tokens any of its rows sees: [lo, hi)
-    int c0, units;   // first chunk; chunks, and kTileCost units more
+    int c0, units;   // first chunk; chunks, and COST units more
 };
 
-// What beginning and ending a tile costs, in units (preparing queries, joining
-// warps: 4 us, where a unit of 128 tokens takes 2.5 us): a tile's first
-// kTileCost units stand for it and hold no tokens, so that a CTA with many
-// short tiles gets fewer tokens. Without them 64 sequences of up to 8191
-// tokens took 138 us, CTAs with 12 tiles ending at 137, the median at 101.
-constexpr int kTileCost = 2;
+// COST: what beginning and ending a tile costs, in units. A tile's first COST
+// units stand for it and hold no tokens, so that a CTA with many short tiles
+// gets fewer tokens. (Few columns: preparing queries and joining warps takes
+// 4 us where a unit of 128 tokens takes 2.5; without the charge 64 sequences
+// of up to 8191 tokens took 138 us, CTAs with 12 tiles ending at 137 and the
+// median at 101.)
 
 // One past the last token row i sees, 0 for a row that sees nothing.
 __device__ __forceinline__ int kv_row_end(const KvArgs& c, const KvAttn& a, int i, int seq) {
@@ -85,7 +85,7 @@ __device__ __forceinline__ int kv_row_end(const KvArgs& c, const KvAttn& a, int 
 
 // The segment that starts at row i, if one does (else rows = 0). Rows of a
 // negative sequence belong to none.
-template <int CH>
+template <int CH, int COST>
 __device__ __forceinline__ KvSegment kv_segment(const KvArgs& c, const KvAttn& a, int i) {
     KvSegment s;
     s.row = i;
@@ -106,14 +106,14 @@ __device__ __forceinline__ KvSegment kv_segment(const KvArgs& c, const KvAttn& a
     if (s.hi == 0) s.lo = 0;
     s.c0 = s.lo / CH;
     // a segment that sees nothing is still one unit: its rows are written
-    s.units = max(1, (s.hi + CH - 1) / CH - s.c0) + kTileCost;
+    s.units = max(1, (s.hi + CH - 1) / CH - s.c0) + COST;
     return s;
 }
 
 // The units a CTA owns, walked segment by segment: of `total` units CTA c gets
 // `each`, the first `extra` CTAs one more. Units are counted in 32 bits (the
 // host cuts calls that could have more into several).
-template <int CH, int THREADS>
+template <int CH, int COST, int THREADS>
 struct KvWalk {
     unsigned begin, end;   // this CTA's units
     unsigned each, extra;
@@ -135,7 +135,7 @@ struct KvWalk {
         KvSegment first;
         first.rows = 0;
         for (int i = i0; i < i1; i++) {
-            const KvSegment s = kv_segment<CH>(c, a, i);
+            const KvSegment s = kv_segment<CH, COST>(c, a, i);
             if (s.rows) mine += (unsigned)(s.units * tiles);
             if (s.rows && !first.rows) first = s;
         }
@@ -163,7 +163,7 @@ struct KvWalk {
         if (begin >= before && begin < before + mine) {
             // this thread's strip holds the first unit
             for (int i = first.row;; i++) {
-                const KvSegment s = i == first.row ? first : kv_segment<CH>(c, a, i);
+                const KvSegment s = i == first.row ? first : kv_segment<CH, COST>(c, a, i);
                 if (!s.rows) continue;
                 const unsigned u = (unsigned)(s.units * tiles);
                 if (begin < before + u) {
@@ -185,78 +185,12 @@ struct KvWalk {
         base += (unsigned)(seg.units * c.nkv * a.subs);
         int i = seg.row + seg.rows;
         while (i < a.n) {
-            seg = kv_segment<CH>(c, a, i);
+            seg = kv_segment<CH, COST>(c, a, i);
             if (seg.rows) return;
             i++;
         }
     }
 };
-
-// One CTA per (row, query head), four warps on alternating tokens, lanes over
-// the head's dims; each warp keeps the running maximum, sum and weighted sum
-// of a softmax in f32, joined at the end.
-template <int DT>
-__global__ void __launch_bounds__(128) kv_attention_kernel(KvArgs c, KvAttn a) {
-    __shared__ float s_m[4], s_l[4], s_o[4][256];
-    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int seq = a.seqs ? a.seqs[row] : 0, head = h / a.group;
-    if (seq < 0) return;
-    int end = a.positions[row] + 1;
-    if (seq >= c.n_seqs || end > c.capacity()) {
-        if (threadIdx.x == 0) raise_error(c.err, kErrBounds);
-        end = 0;
-    }
-    const int begin = a.window > 0 ? max(0, end - a.window) : 0;
-    float q[8], o[8], m = -__int_as_float(0x7f800000), l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int d = lane + 32 * i;
-        q[i] = d < c.hd ? load1<DT>(a.q, (size_t)row * a.q_stride + (size_t)h * c.hd + d) : 0.0f;
-        o[i] = 0.0f;
-    }
-    for (int t = begin + warp; t < end; t += 4) {
-        const int page = c.page_of(c.table, seq, t), slot = c.slot(t);
-        if (page < 0) {
-            raise_error(c.err, kErrBounds);
-            continue;
-        }
-        const size_t at = c.code_at(page, head, slot), sa = c.scale_at(page, head, slot);
-        float s = 0.0f, v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = lane + 32 * i;
-            const bool in = d < c.hd;
-            s = fmaf(q[i], in ? (float)c.k[at + d] : 0.0f, s);
-            v[i] = in ? (float)c.v[at + d] : 0.0f;
-        }
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= c.ks[sa] * a.scale;
-        const float top = fmaxf(m, s), fix = expf(m - top), p = expf(s - top), f = p * c.vs[sa];
-        l = l * fix + p;
-        m = top;
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = fmaf(f, v[i], o[i] * fix);
-    }
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-#pragma unroll
-    for (int i = 0; i < 8; i++) s_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), sum = 0.0f, f[4];
-    const bool empty = !(top > -__int_as_float(0x7f800000)) && top == top;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        f[w] = empty || s_l[w] == 0.0f ? 0.0f : expf(s_m[w] - top);
-        sum += f[w] * s_l[w];
-    }
-    for (int d = threadIdx.x; d < c.hd; d += 128) {
-        float x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) x += f[w] * s_o[w][d];
-        store1<DT>(a.out, (size_t)row * a.out_stride + (size_t)h * c.hd + d, empty ? 0.0f : x / sum);
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[(size_t)row * a.nh + h] = empty ? -__int_as_float(0x7f800000) : top + logf(sum);
-}
 
 // ---------------------------------------------------------------------------
 // small matrix pieces
@@ -427,7 +361,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(KvAttn a, int hd,
 // so that the fragments' loads meet no bank twice. Whatever bytes lie in a
 // hidden token or behind the head's dims, they are finite codes, and the
 // token's weight, like a missing dim of q, is 0.
-constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
+constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewCost = 2;
 
 template <int DP>
 struct FewCfg {
@@ -479,7 +413,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
     const float none = -__int_as_float(0x7f800000);
 
     if (tid == 0) a.splits[blockIdx.x].parts = 0;
-    KvWalk<CH, kFewThreads> walk;
+    KvWalk<CH, kFewCost, kFewThreads> walk;
     if (!walk.start(c, a, &s_seg, s_sum)) return;
     unsigned unit = walk.begin;
     while (unit < walk.end) {
@@ -487,7 +421,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         const KvSegment seg = walk.seg;
         const int tile = (int)((unit - walk.base) / (unsigned)seg.units), head = tile / a.subs, sub = tile - head * a.subs;
         const unsigned tile0 = walk.base + (unsigned)(tile * seg.units), tile1 = tile0 + seg.units;
-        const unsigned first = tile0 + kTileCost;  // the tile's first chunk
+        const unsigned first = tile0 + kFewCost;  // the tile's first chunk
         if (walk.end <= first) return;             // this CTA's units end before it
         const unsigned from = max(unit, first);
         const int u0 = seg.c0 + (int)(from - first), u1 = seg.c0 + (int)(min(tile1, walk.end) - first);
@@ -897,6 +831,396 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
         if (split && tid < cols) {
             part[tid] = s_f[tid];
             part[COLS + tid] = s_inv[tid];
+        }
+        if (split && first >= walk.begin && tid == 0)
+            a.splits[blockIdx.x] = {(int)walk.owner(tile1 - 1) - (int)blockIdx.x + 1, cols, heads, seg.row, h0};
+        __syncthreads();
+        unit = min(tile1, walk.end);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// many columns: 64 of them per tile, codes widened to f16 once for all
+//
+// Four warps of 16 columns each. A unit of UT tokens arrives as codes by
+// asynchronous copies (one unit ahead), is widened to f16 tiles in shared
+// memory by all warps, and feeds both products from there: S = q K^T with q
+// from shared memory, O += P V with P straight from S's registers. q is scaled
+// by a power of two to at most 2^14: exact in f16 for f16 and (down to 2^-38
+// of the row's largest value) bf16, two f16 (22 bits) for f32. Tiles lie in
+// rows of 2 DP bytes whose 16-byte pieces are xor-ed with the row's number, so
+// that neither the stores nor the matrix loads meet a bank twice.
+// Bound by the matrix instructions (m16n8k16 issues once in 8 cycles).
+// ---------------------------------------------------------------------------
+constexpr int kManyWarps = 4, kManyThreads = 32 * kManyWarps, kManyCols = 16 * kManyWarps, kManyCost = 2;
+
+template <int DT, int DP>
+struct ManyCfg {
+    static constexpr int SPLIT = DT == 0 ? 2 : 1;
+    static constexpr int UT = DP <= 128 ? 64 : 32;        // tokens of a unit
+    static constexpr int CODES = UT * DP;                 // bytes of a unit's keys (or values)
+    static constexpr int QUERY = kManyCols * DP * 2;      // one f16 part of the queries
+    static constexpr int TILE = UT * DP * 2;              // f16 keys (or values)
+    static constexpr int SMEM = SPLIT * QUERY + 2 * TILE + 4 * CODES;
+    static constexpr int PER_SM = DP == 256 && SPLIT == 2 ? 1 : 2;
+};
+
+__device__ __forceinline__ void load_matrix(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void load_matrix_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void store_shared16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// Four codes as four f16 in order.
+__device__ __forceinline__ uint2 codes_f16(uint32_t w) {
+    const uint32_t x = w ^ 0x80808080u, off = 0x64806480u;
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 o = *reinterpret_cast<const __half2*>(&off);
+    const __half2 h0 = __hsub2(*reinterpret_cast<const __half2*>(&a), o), h1 = __hsub2(*reinterpret_cast<const __half2*>(&b), o);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+}
+// Power of two that brings amax to at most 2^14 and at least 2^13.
+__device__ __forceinline__ float kv_query_scale_f16(float amax) {
+    if (!(amax > 0.0f) || !(amax <= 0x1.fffffep127f)) return 1.0f;
+    int e;
+    frexpf(amax, &e);
+    return ldexpf(1.0f, min(126, max(-126, 14 - e)));
+}
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn_many_kernel(KvArgs c, KvAttn a) {
+    using Cfg = ManyCfg<DT, DP>;
+    constexpr int UT = Cfg::UT, SPLIT = Cfg::SPLIT, NB = UT / 16, ROW = 2 * DP;
+    constexpr int PIECES = DP / 16;                     // 16-byte pieces of a row of codes
+    constexpr int STEP = kManyThreads / PIECES;         // rows the CTA copies at once
+    __shared__ KvSegment s_seg;
+    __shared__ unsigned s_sum[kManyWarps + 1];
+    __shared__ float s_up[kManyCols];
+    __shared__ int s_end[kManyCols];
+    __shared__ FewBlock s_block[2][NB];
+    extern __shared__ __align__(128) int8_t s_many[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+    const int hd = c.hd;
+    const float none = -__int_as_float(0x7f800000);
+    const uint32_t s_q = smem_addr(s_many), s_k = s_q + SPLIT * Cfg::QUERY, s_v = s_k + Cfg::TILE, s_codes = s_v + Cfg::TILE;
+
+    if (tid == 0) a.splits[blockIdx.x].parts = 0;
+    KvWalk<UT, kManyCost, kManyThreads> walk;
+    if (!walk.start(c, a, &s_seg, s_sum)) return;
+    unsigned unit = walk.begin;
+    while (unit < walk.end) {
+        while (unit >= walk.base + (unsigned)(walk.seg.units * c.nkv * a.subs)) walk.next(c, a);
+        const KvSegment seg = walk.seg;
+        const int tile = (int)((unit - walk.base) / (unsigned)seg.units), head = tile / a.subs, sub = tile - head * a.subs;
+        const unsigned tile0 = walk.base + (unsigned)(tile * seg.units), tile1 = tile0 + seg.units;
+        const unsigned first = tile0 + kManyCost;  // the tile's first chunk
+        if (walk.end <= first) return;             // this CTA's units end before it
+        const unsigned from = max(unit, first);
+        const int u0 = seg.c0 + (int)(from - first), u1 = seg.c0 + (int)(min(tile1, walk.end) - first);
+        const int heads = min(a.heads, a.group - sub * a.heads), cols = seg.rows * heads;
+        const int h0 = head * a.group + sub * a.heads;
+
+        // ---- copies of a unit's codes: thread -> (row, piece), rows STEP apart ----
+        const unsigned page_codes = (unsigned)(c.nkv * hd) << c.page_log2, page_scales = (unsigned)c.nkv << c.page_log2 >> 4;
+        const int my_row = tid / PIECES, my_piece = tid % PIECES;
+        const bool copies = 16 * my_piece < hd;
+        const size_t my_at = ((size_t)head << c.page_log2) * hd + 16 * my_piece;
+        const float* ksbase = c.ks + ((size_t)head << c.page_log2 >> 4);
+        const float* vsbase = c.vs + ((size_t)head << c.page_log2 >> 4);
+        const int32_t* row = c.table + (size_t)min(seg.seq, c.n_seqs - 1) * c.max_pages;
+        // pages of 32 blocks by lane, the next 32 under way (as above)
+        auto find = [&](int u) {
+            const int t = u * UT + 16 * lane;
+            int pg = -1;
+            if (t < u1 * UT && t < seg.hi && t + 16 > seg.lo) {
+                pg = c.checked(row[t >> c.page_log2]);
+                if (pg < 0 && warp == 0) raise_error(c.err, kErrBounds);
+            }
+            return pg;
+        };
+        constexpr int HELD = 32 / NB;  // units whose pages are held
+        int pages = find(u0), pages_next = find(u0 + HELD), pages_from = u0;
+        auto fetch = [&](int u) {
+            if (u < u1) {
+                if (u - pages_from == HELD) {
+                    pages = pages_next;
+                    pages_from = u;
+                    pages_next = find(u + HELD);
+                }
+                const int stage = (u - u0) & 1;
+                const uint32_t dst = s_codes + stage * 2 * Cfg::CODES + 16 * tid;
+#pragma unroll
+                for (int r = 0; r < UT; r += STEP) {
+                    // a warp's rows lie in one block
+                    const int b = (r + my_row) >> 4;
+                    const int pg = __shfl_sync(0xffffffffu, pages, (u - pages_from) * NB + b);
+                    if (pg < 0 || !copies) continue;
+                    const int slot = c.slot(u * UT + r + my_row);
+                    const size_t at = (size_t)(unsigned)pg * page_codes + (unsigned)(slot * hd) + my_at;
+                    cp_async16(dst + r * DP, c.k + at);
+                    cp_async16(dst + Cfg::CODES + r * DP, c.v + at);
+                }
+                const int pg = __shfl_sync(0xffffffffu, pages, (u - pages_from) * NB + (tid & (NB - 1)));
+                if (tid < NB) {
+                    FewBlock& block = s_block[stage][tid];
+                    block.page = pg;
+                    if (pg >= 0) {
+                        const size_t sa = (size_t)(unsigned)pg * page_scales + (c.slot(u * UT + 16 * tid) >> 4);
+                        cp_async4(smem_addr(&block.ks), ksbase + sa);
+                        cp_async4(smem_addr(&block.vs), vsbase + sa);
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+        fetch(u0);
+
+        // ---- queries: a warp widens its own 16 columns ----
+        for (int k = 16 * warp; k < 16 * warp + 16; k++) {
+            float amax = 0.0f, x[(DP + 127) / 128][4];
+            bool wild = false;
+            const size_t at = k < cols ? (size_t)(seg.row + k / heads) * a.q_stride + (size_t)(h0 + k % heads) * hd : 0;
+#pragma unroll
+            for (int v = 0; v < (DP + 127) / 128; v++) {
+                const int d = 128 * v + 4 * lane;
+                x[v][0] = x[v][1] = x[v][2] = x[v][3] = 0.0f;
+                if (k < cols && d < hd) load4<DT>(a.q, at + d, x[v]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    amax = fmaxf(amax, fabsf(x[v][i]));
+                    wild |= !(fabsf(x[v][i]) <= 0x1.fffffep127f);
+                }
+            }
+            const float up = kv_query_scale_f16(warp_max_abs(amax));
+            wild = __any_sync(0xffffffffu, wild);
+#pragma unroll
+            for (int v = 0; v < (DP + 127) / 128; v++) {
+                const int d = 128 * v + 4 * lane;
+                if (d >= DP) continue;
+#pragma unroll
+                for (int z = 0; z < SPLIT; z++) {
+                    uint32_t w[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        float y0 = x[v][2 * i] * up, y1 = x[v][2 * i + 1] * up;
+                        if (z) {
+                            y0 -= __half2float(__float2half_rn(y0));
+                            y1 -= __half2float(__float2half_rn(y1));
+                        }
+                        w[i] = pack_f16(y0, y1);
+                    }
+                    const uint32_t to = s_q + z * Cfg::QUERY + k * ROW + 16 * ((d >> 3) ^ (k & 7)) + 2 * (d & 7);
+                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(w[0]), "r"(w[1]) : "memory");
+                }
+            }
+            if (lane == 0) {
+                s_up[k] = wild ? __int_as_float(0x7fc00000) : a.scale * kLog2e / up;  // NaN: so are the column's scores
+                int end = 0;
+                if (k < cols) {
+                    const int p = a.positions[seg.row + k / heads];
+                    end = p >= 0 && p < seg.hi ? p + 1 : 0;
+                }
+                s_end[k] = end;
+            }
+        }
+        __syncwarp();
+        // a lane's columns of the products: 16 warp + g, + 8
+        float qs[2], m[2], l[2], acc[DP / 8][4];
+        int end[2], begin[2], all_lo = 0, all_hi = INT_MAX, any_hi = 0;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int k = 16 * warp + g + 8 * e;
+            qs[e] = s_up[k];
+            end[e] = s_end[k];
+            begin[e] = a.window > 0 ? max(0, end[e] - a.window) : 0;
+            m[e] = none;
+            l[e] = 0.0f;
+            if (k < cols) {
+                all_hi = min(all_hi, end[e]);
+                all_lo = max(all_lo, begin[e]);
+                any_hi = max(any_hi, end[e]);
+            }
+        }
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        any_hi = __reduce_max_sync(0xffffffffu, any_hi);
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+        float vtop = 0.0f, vinv = 0.0f;
+
+        for (int u = u0; u < u1; u++) {
+            const int t0 = u * UT, stage = (u - u0) & 1;
+            cp_async_wait<0>();
+            __syncthreads();  // the codes are there, and no one reads the tiles any more
+            fetch(u + 1);
+#pragma unroll
+            for (int r = 0; r < UT; r += STEP) {
+                const int t = r + my_row, odd = my_piece >> 2 & 1;
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const uint4 x = load_shared16(s_codes + (2 * stage + v) * Cfg::CODES + 16 * tid + r * DP);
+                    const uint2 h0 = codes_f16(x.x), h1 = codes_f16(x.y), h2 = codes_f16(x.z), h3 = codes_f16(x.w);
+                    const uint4 lo = make_uint4(h0.x, h0.y, h1.x, h1.y), hi = make_uint4(h2.x, h2.y, h3.x, h3.y);
+                    const uint32_t to = (v ? s_v : s_k) + t * ROW;
+                    store_shared16(to + 16 * ((2 * my_piece + odd) ^ (t & 7)), odd ? hi : lo);
+                    store_shared16(to + 16 * ((2 * my_piece + 1 - odd) ^ (t & 7)), odd ? lo : hi);
+                }
+            }
+            __syncthreads();
+            if (t0 >= any_hi || t0 + UT <= seg.lo) continue;  // nothing of it for this warp's columns
+
+            // ---- S = q K^T ----
+            float s[UT / 8][4];
+#pragma unroll
+            for (int i = 0; i < UT / 8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < DP / 16; p++) {
+                uint32_t q[SPLIT][4];
+#pragma unroll
+                for (int z = 0; z < SPLIT; z++) {
+                    const int r = 16 * warp + (lane & 15);
+                    load_matrix(q[z], s_q + z * Cfg::QUERY + r * ROW + 16 * ((2 * p + (lane >> 4)) ^ (r & 7)));
+                }
+#pragma unroll
+                for (int i = 0; i < UT / 16; i++) {
+                    uint32_t k[4];
+                    const int t = 16 * i + (lane & 7) + (lane >> 4 << 3);
+                    load_matrix(k, s_k + t * ROW + 16 * ((2 * p + (lane >> 3 & 1)) ^ (t & 7)));
+#pragma unroll
+                    for (int z = 0; z < SPLIT; z++) {
+                        mma_f16(s[2 * i], q[z][0], q[z][1], q[z][2], q[z][3], k[0], k[1]);
+                        mma_f16(s[2 * i + 1], q[z][0], q[z][1], q[z][2], q[z][3], k[2], k[3]);
+                    }
+                }
+            }
+            // ---- softmax: score = s f in units of log 2 ----
+            float ks[NB], vs[NB];
+            int page[NB];
+            bool whole = t0 >= all_lo && t0 + UT <= all_hi;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const FewBlock block = s_block[stage][b];
+                const int t = t0 + 16 * b;
+                const bool none_of_it = block.page < 0 || t >= seg.hi || t + 16 <= seg.lo;
+                page[b] = none_of_it ? -1 : block.page;
+                ks[b] = none_of_it ? 0.0f : block.ks;
+                vs[b] = none_of_it ? 0.0f : block.vs;
+                whole = whole && !none_of_it;
+            }
+            unsigned hidden[2] = {0, 0};  // bit 2 i + e & 1 of token 8 i + 2 q4 + (e & 1)
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < UT / 8; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int t = t0 + 8 * i + 2 * q4 + (e & 1);
+                        if (page[i / 2] < 0 || t >= end[e >> 1] || t < begin[e >> 1]) hidden[e >> 1] |= 1u << (2 * i + (e & 1));
+                    }
+            }
+            float top[2] = {m[0], m[1]}, vmax = vtop;
+#pragma unroll
+            for (int b = 0; b < NB; b++) vmax = fmaxf(vmax, vs[b]);
+#pragma unroll
+            for (int i = 0; i < UT / 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y = s[i][e] * (ks[i / 2] * qs[e >> 1]);
+                    top[e >> 1] = fmaxf(top[e >> 1], hidden[e >> 1] >> (2 * i + (e & 1)) & 1u ? none : y);
+                }
+            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || vmax > vtop)) {
+                const float fix_v = vmax > 0.0f ? vtop / vmax : 1.0f;
+                vtop = vmax;
+                vinv = vmax > 0.0f ? kWeightTop / vmax : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float x = top[e];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    const float fix = m[e] == none ? 0.0f : exp2_fast(m[e] - x);
+                    m[e] = x;
+                    l[e] *= fix;
+#pragma unroll
+                    for (int i = 0; i < DP / 8; i++) {
+                        acc[i][2 * e] *= fix * fix_v;
+                        acc[i][2 * e + 1] *= fix * fix_v;
+                    }
+                }
+            }
+            const float base[2] = {m[0] == none ? 0.0f : m[0], m[1] == none ? 0.0f : m[1]};
+            // ---- O += P V, 16 tokens (a block) at a time ----
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const float fv = vs[b] * vinv;
+                uint32_t p[SPLIT][4];  // A fragment: (g, 2 q4), (g + 8, ..), (g, 2 q4 + 8), ..
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int i = 2 * b + j;
+                        float x = exp2_fast(fmaf(s[i][e], ks[b] * qs[e >> 1], -base[e >> 1]));
+                        if (hidden[e >> 1] >> (2 * i + (e & 1)) & 1u) x = 0.0f;
+                        l[e >> 1] += x;
+                        w[e] = x * fv;
+                    }
+                    p[0][2 * j] = pack_f16(w[0], w[1]);
+                    p[0][2 * j + 1] = pack_f16(w[2], w[3]);
+                    if (SPLIT == 2) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] -= __half2float(__float2half_rn(w[e]));
+                        p[SPLIT - 1][2 * j] = pack_f16(w[0], w[1]);
+                        p[SPLIT - 1][2 * j + 1] = pack_f16(w[2], w[3]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) {
+                    uint32_t v[4];
+                    const int t = 16 * b + (lane & 15);
+                    load_matrix_t(v, s_v + t * ROW + 16 * ((2 * i + (lane >> 4)) ^ (t & 7)));
+#pragma unroll
+                    for (int z = 0; z < SPLIT; z++) {
+                        mma_f16(acc[2 * i], p[z][0], p[z][1], p[z][2], p[z][3], v[0], v[1]);
+                        mma_f16(acc[2 * i + 1], p[z][0], p[z][1], p[z][2], p[z][3], v[2], v[3]);
+                    }
+                }
+            }
+        }
+        cp_async_wait<0>();
+
+        // ---- a warp's columns are its own: finished, or a part of a split tile ----
+        const bool split = first < walk.begin || tile1 > walk.end;
+        const float unscale = vtop / kWeightTop;
+        float* part = a.parts + ((size_t)2 * blockIdx.x + (first >= walk.begin)) * a.part_floats;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float sum = l[e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int k = 16 * warp + g + 8 * e;
+#pragma unroll
+            for (int i = 0; i < DP / 8; i++) {
+                // a quad's lanes trade pairs, so that each holds four dims in a row
+                const float x0 = acc[i][2 * e] * unscale, x1 = acc[i][2 * e + 1] * unscale;
+                const float y0 = __shfl_xor_sync(0xffffffffu, x0, 1), y1 = __shfl_xor_sync(0xffffffffu, x1, 1);
+                const int d = 8 * i + 2 * (q4 & 2);
+                if (k >= cols || d >= hd || (q4 & 1) != (i & 1)) continue;
+                float x[4] = {q4 & 1 ? y0 : x0, q4 & 1 ? y1 : x1, q4 & 1 ? x0 : y0, q4 & 1 ? x1 : y1};
+                if (split) *reinterpret_cast<float4*>(part + 2 * kManyCols + (size_t)k * hd + d) = make_float4(x[0], x[1], x[2], x[3]);
+                else kv_finish<DT>(a, seg.row + k / heads, h0 + k % heads, hd, d, x, m[e], sum);
+            }
+            if (split && q4 == 0 && k < cols) {
+                part[k] = m[e];
+                part[kManyCols + k] = sum;
+            }
         }
         if (split && first >= walk.begin && tid == 0)
             a.splits[blockIdx.x] = {(int)walk.owner(tile1 - 1) - (int)blockIdx.x + 1, cols, heads, seg.row, h0};

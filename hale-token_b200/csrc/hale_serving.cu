@@ -139,15 +139,15 @@ hale_status check_layer_rows(hale_ctx* ctx, const hale_kv8* kv, const char* what
 
 // CTAs of an attention launch: what the GPU holds at once, no more than there
 // can be units of CH tokens, and no more than the workspace has parts for.
-unsigned attn_grid(const hale_ctx* ctx, const KvArgs& c, const KvAttn& a, int per_sm, int chunk) {
-    const uint64_t units = (uint64_t)a.n * c.nkv * a.subs * ((uint64_t)c.capacity() / chunk + 1 + kTileCost);
+unsigned attn_grid(const hale_ctx* ctx, const KvArgs& c, const KvAttn& a, int per_sm, int chunk, int cost) {
+    const uint64_t units = (uint64_t)a.n * c.nkv * a.subs * ((uint64_t)c.capacity() / chunk + 1 + cost);
     const uint64_t parts = kAttnPartBytes / 8 / a.part_floats;
     return (unsigned)std::min<uint64_t>({(uint64_t)ctx->sm_count * per_sm, units, parts, (uint64_t)kAttnMaxGrid});
 }
 
 // Rows of one launch: units are counted in 32 bits.
-uint32_t attn_rows(const KvArgs& c, const KvAttn& a, int chunk) {
-    const uint64_t row = (uint64_t)c.nkv * a.subs * ((uint64_t)c.capacity() / chunk + 1 + kTileCost);
+uint32_t attn_rows(const KvArgs& c, const KvAttn& a, int chunk, int cost) {
+    const uint64_t row = (uint64_t)c.nkv * a.subs * ((uint64_t)c.capacity() / chunk + 1 + cost);
     const uint64_t rows = std::max<uint64_t>(1, 0x7fffffffull / row) / a.rows * a.rows;
     return (uint32_t)std::min<uint64_t>((uint64_t)a.n, std::max<uint64_t>(rows, (uint64_t)a.rows));
 }
@@ -193,13 +193,32 @@ hale_status attn_few(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cud
     a.part_floats = cols * (2 + c.hd);
     const size_t smem = std::max((size_t)kFewWarps * cols * DP * 4, (size_t)kFewWarps * FewCfg<DP>::RING);
     CUDA_TRY(ctx, allow_smem(kv_attn_few_kernel<DT, DP, HD, NT>, smem));
-    const uint32_t step = attn_rows(c, a, FewCfg<DP>::CH), n = (uint32_t)a.n;
+    const uint32_t step = attn_rows(c, a, FewCfg<DP>::CH, kFewCost), n = (uint32_t)a.n;
     for (uint32_t i = 0; i < n; i += step) {
         const KvAttn b = attn_part<DT>(a, i, std::min(step, n - i));
-        const unsigned grid = attn_grid(ctx, c, b, DP <= 128 && NT == 1 ? 3 : 2, FewCfg<DP>::CH);
+        const unsigned grid = attn_grid(ctx, c, b, DP <= 128 && NT == 1 ? 3 : 2, FewCfg<DP>::CH, kFewCost);
         kv_attn_few_kernel<DT, DP, HD, NT><<<grid, kFewThreads, smem, st>>>(c, b);
         if (hale_status r = check_launch(ctx, "kv_attn_few")) return r;
         if (hale_status r = attn_join<DT>(ctx, b, c.hd, cols, grid, st)) return r;
+    }
+    return HALE_OK;
+}
+
+template <int DT, int DP>
+hale_status attn_many(hale_ctx* ctx, const KvArgs& c, KvAttn a, uint32_t run, cudaStream_t st) {
+    using Cfg = ManyCfg<DT, DP>;
+    a.heads = std::min(a.group, kManyCols);
+    a.subs = (a.group + a.heads - 1) / a.heads;
+    a.rows = (int)std::max<uint32_t>(1u, std::min<uint32_t>(run, (uint32_t)(kManyCols / a.heads)));
+    a.part_floats = kManyCols * (2 + c.hd);
+    CUDA_TRY(ctx, allow_smem(kv_attn_many_kernel<DT, DP>, Cfg::SMEM));
+    const uint32_t step = attn_rows(c, a, Cfg::UT, kManyCost), n = (uint32_t)a.n;
+    for (uint32_t i = 0; i < n; i += step) {
+        const KvAttn b = attn_part<DT>(a, i, std::min(step, n - i));
+        const unsigned grid = attn_grid(ctx, c, b, Cfg::PER_SM, Cfg::UT, kManyCost);
+        kv_attn_many_kernel<DT, DP><<<grid, kManyThreads, Cfg::SMEM, st>>>(c, b);
+        if (hale_status r = check_launch(ctx, "kv_attn_many")) return r;
+        if (hale_status r = attn_join<DT>(ctx, b, c.hd, kManyCols, grid, st)) return r;
     }
     return HALE_OK;
 }
@@ -224,8 +243,9 @@ hale_status attn_go(hale_ctx* ctx, const KvArgs& c, const KvAttn& a, uint32_t ru
         default: return attn_few<DT, 128, 0, 2>(ctx, c, a, run, st);
         }
     }
-    kv_attention_kernel<DT><<<dim3(a.n, a.nh), 128, 0, st>>>(c, a);
-    return check_launch(ctx, "kv_attention");
+    if (c.hd <= 64) return attn_many<DT, 64>(ctx, c, a, run, st);
+    if (c.hd <= 128) return attn_many<DT, 128>(ctx, c, a, run, st);
+    return attn_many<DT, 256>(ctx, c, a, run, st);
 }
 
 template <int DT>

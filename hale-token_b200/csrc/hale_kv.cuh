@@ -164,15 +164,28 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvArgs c, KvAppend a) {
     __syncthreads();
     const int blocks = s_n;
     if (blocks == 0) return;
-    for (int i = tid; i < a.n; i += 256) {
-        const long long key = kv_row_key(c, a, i);
-        if (key < 0) continue;
+    auto look = [&](int i, int seq, int pos) {
+        if (seq < 0 || pos < 0) return;
+        const long long key = ((long long)seq << 32) | (unsigned)(pos / kKvBlock);
         for (int b = 0; b < blocks; b++) {
             if (s_key[b] != key) continue;
             if (i < s_first[b]) s_late[b] = 1;  // an earlier row leads this block
-            else atomicMax(&s_slot[b][a.positions[i] % kKvBlock], i);
+            else atomicMax(&s_slot[b][pos % kKvBlock], i);
         }
+    };
+    // four rows a load where both lists start on 16-byte boundaries
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.seqs) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
+    const int n4 = vec ? a.n & ~3 : 0;
+#pragma unroll 2
+    for (int i = 4 * tid; i < n4; i += 4 * 256) {
+        const int4 p = *reinterpret_cast<const int4*>(a.positions + i);
+        const int4 s = a.seqs ? *reinterpret_cast<const int4*>(a.seqs + i) : make_int4(0, 0, 0, 0);
+        look(i, s.x, p.x);
+        look(i + 1, s.y, p.y);
+        look(i + 2, s.z, p.z);
+        look(i + 3, s.w, p.w);
     }
+    for (int i = n4 + tid; i < a.n; i += 256) look(i, a.seqs ? a.seqs[i] : 0, a.positions[i]);
     __syncthreads();
     const int tasks = blocks * c.nkv * 2, step = 8 * gridDim.y;
     for (int t = warp + 8 * blockIdx.y; t < tasks; t += step) {

@@ -276,8 +276,8 @@ extern "C" hale_status hale_kv8_append(hale_ctx* ctx, const hale_kv8* kv, uint32
     // of 8 heads: 128 CTAs). In long lists 15 of 16 such CTAs would lead no
     // block, and every one of them reads the whole list: 32 rows then.
     if (n > 1024) a.rows_per_cta = kAppendRows;
-    const uint32_t blocks = a.rows_per_cta == 1 ? 1 : 3;
-    const dim3 grid((n + a.rows_per_cta - 1) / a.rows_per_cta, std::min(64u, (2 * c.nkv * blocks + 7) / 8));
+    const dim3 grid((n + a.rows_per_cta - 1) / a.rows_per_cta,
+                    a.rows_per_cta == 1 ? std::min(64u, (2u * c.nkv + 7) / 8) : 1u);
     ProfScope ps(ctx, "kv8_append", S(stream));
     switch (dtype) {
     case HALE_F32: append_go<0>(c, a, grid, S(stream)); break;
@@ -487,8 +487,8 @@ extern "C" hale_status hale_verify_drafts(hale_ctx* ctx, const void* logits, hal
         return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: temperature is not finite", what);
     if (max_draft > (uint32_t)kVerifyMaxDraft)
         return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: %u drafted tokens (up to %d)", what, max_draft, kVerifyMaxDraft);
-    // 8 CTAs note the mass of each 256 values in shared memory: 2^24 values are 64 KB
-    if (vocab == 0 || vocab > (1u << 24)) return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: vocab %u out of range", what, vocab);
+    // a CTA notes the mass of each 256 values in shared memory: 2^22 values are 128 KB
+    if (vocab == 0 || vocab > (1u << 22)) return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: vocab %u out of range", what, vocab);
     if (logits_stride < vocab || (draft_probs && probs_stride < vocab) || logits_stride > (1ull << 40) ||
         probs_stride > (1ull << 40))
         return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: rows are closer together than the vocabulary is long", what);
@@ -534,23 +534,24 @@ extern "C" hale_status hale_verify_drafts(hale_ctx* ctx, const void* logits, hal
         }
     }
     if ((r = check_launch(ctx, "verify_stats"))) return r;
-    const size_t smem = ((size_t)(vocab + kPickTile - 1) / kPickTile / kVerifyCluster + 1) * 8;
+    // clusters of 8 CTAs, of fewer where the GPU would not hold them all at once
+    // (two CTAs an SM)
+    const unsigned ctas = std::max(1u, std::min((unsigned)kVerifyCluster, 2u * ctx->sm_count / batch));
+    const size_t smem = (((size_t)vocab + kPickTile - 1) / kPickTile / ctas + 1) * 8;
     ProfScope ps(ctx, "verify_pick", st);
-    const unsigned pick = batch * kVerifyCluster;
-    switch (dtype) {
-    case HALE_F32:
-        CUDA_TRY(ctx, allow_smem(verify_pick_kernel<0>, smem));
-        verify_pick_kernel<0><<<pick, kPickThreads, smem, st>>>(a);
-        break;
-    case HALE_F16:
-        CUDA_TRY(ctx, allow_smem(verify_pick_kernel<1>, smem));
-        verify_pick_kernel<1><<<pick, kPickThreads, smem, st>>>(a);
-        break;
-    default:
-        CUDA_TRY(ctx, allow_smem(verify_pick_kernel<2>, smem));
-        verify_pick_kernel<2><<<pick, kPickThreads, smem, st>>>(a);
-        break;
-    }
+    auto pick = dtype == HALE_F32 ? verify_pick_kernel<0> : dtype == HALE_F16 ? verify_pick_kernel<1> : verify_pick_kernel<2>;
+    CUDA_TRY(ctx, allow_smem(pick, smem));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(batch * ctas);
+    cfg.blockDim = dim3(kPickThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute shape{};
+    shape.id = cudaLaunchAttributeClusterDimension;
+    shape.val.clusterDim = {ctas, 1, 1};
+    cfg.attrs = &shape;
+    cfg.numAttrs = 1;
+    CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, pick, a));
     return check_launch(ctx, "verify_pick");
 } catch (...) {
     return HALE_E_OUT_OF_MEMORY;

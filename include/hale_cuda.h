@@ -645,7 +645,7 @@ HALE_API hale_status hale_kv8_copy(hale_ctx* ctx, const hale_kv8* kv, const int3
  * the logits), 0 behind them. A row with nothing above -infinity keeps nothing
  * and draws nothing. A drafted token outside the vocabulary, or a count
  * outside 0 .. max_draft, is not kept and reported as HALE_E_DEVICE_CHECK.
- * batch * (max_draft + 1) up to 65535, vocab up to 2^24. */
+ * batch * (max_draft + 1) up to 65535, vocab up to 2^22. */
 HALE_API hale_status hale_verify_drafts(hale_ctx* ctx, const void* logits, hale_dtype dtype, uint64_t logits_stride,
                                         const int32_t* draft_tokens, const float* draft_probs, uint64_t probs_stride,
                                         const int32_t* n_draft, uint32_t batch, uint32_t max_draft, uint32_t vocab,

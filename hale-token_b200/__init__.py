@@ -133,6 +133,8 @@ SIGNATURES = {
     "hale_decoder_forward": (I32, [P, P, U32, U32, P, P, P]),
     "hale_decoder_create_batched": (I32, [P, C.POINTER(DecoderDesc), C.POINTER(DecoderLayer), P, U32, U32, U32,
                                          C.POINTER(P)]),
+    "hale_decoder_create_kv8": (I32, [P, C.POINTER(DecoderDesc), C.POINTER(DecoderLayer), P, U32, U32, C.POINTER(Kv8Struct),
+                                     C.POINTER(P)]),
     "hale_decoder_step": (I32, [P, P, P, P, P, U32, P, I32, P, P]),
     "hale_decoder_generate": (I32, [P, P, P, U32, P, U64, U32, P, U32, P, P, P, P, P]),
     "hale_lm_head": (I32, [P, P, P, U32, P, P]),
@@ -431,10 +433,12 @@ class Decoder:
     v, o and router (MoE layers) or dense_gate / dense_up / dense_down as
     (dtype, rows, cols, encoded uint8 rows). embed, lm_head: (dtype, rows,
     cols, bytes); final_norm: float32 array. pool: the routed experts of the
-    MoE layers in order (pool layer j = j-th MoE layer), or None.
+    MoE layers in order (pool layer j = j-th MoE layer), or None. kv8: a Kv8
+    that holds the keys and values (its sequences are the decoder's) in place
+    of f32 caches.
     """
 
-    def __init__(self, ctx, dims, layers, embed, lm_head, final_norm, pool, max_len, n_seqs=1, max_batch=1):
+    def __init__(self, ctx, dims, layers, embed, lm_head, final_norm, pool, max_len, n_seqs=1, max_batch=1, kv8=None):
         import numpy as np
         self.ctx, self.dims, self._keep = ctx, dict(dims), []
 
@@ -465,8 +469,14 @@ class Decoder:
                            d.get("n_experts", 0), d.get("top_k", 0), int(d.get("normalize_topk", 0)), d["eps"],
                            d["rope_theta"], mat(embed), mat(lm_head), vec(final_norm))
         h = P()
-        ctx.call("hale_decoder_create_batched", ctx.h, C.byref(desc), arr, pool.h if pool is not None else None,
-                 max_len, n_seqs, max_batch, C.byref(h))
+        if kv8 is None:
+            ctx.call("hale_decoder_create_batched", ctx.h, C.byref(desc), arr, pool.h if pool is not None else None,
+                     max_len, n_seqs, max_batch, C.byref(h))
+        else:
+            n_seqs = kv8.n_seqs
+            ctx.call("hale_decoder_create_kv8", ctx.h, C.byref(desc), arr, pool.h if pool is not None else None,
+                     max_len, max_batch, C.byref(kv8.c), C.byref(h))
+        self.kv8 = kv8
         self.n_seqs, self.max_batch, self.max_len = n_seqs, max_batch, max_len
         self.h = h
         self.pool = pool

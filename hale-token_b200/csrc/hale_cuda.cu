@@ -2378,6 +2378,10 @@ struct hale_decoder {
     int32_t* gen_seen = nullptr;
     int32_t* h_tok = nullptr;
     cudaEvent_t gen_ev[3] = {nullptr, nullptr, nullptr};
+    // keys and values in the caller's paged 8-bit cache (hale_decoder_create_kv8)
+    bool paged = false;
+    hale_kv8 kv{};
+    uint32_t kv_run = 1;  // most consecutive rows of one sequence in the step
     // single-row attention over the whole GPU (attn_split_kernel)
     bool split = false;
     int split_grid = 0, split_npm = 0;
@@ -2460,9 +2464,11 @@ static hale_status dec_matrix(hale_ctx* ctx, const hale_host_matrix& m, uint32_t
     return hale_matrix_create(ctx, (hale_dtype)m.dtype, rows, cols, m.data, (uint64_t)rows * rb, 0, out);
 }
 
-extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_decoder_desc* ds,
-                                                   const hale_decoder_layer* lys, hale_pool* pool, uint32_t max_len,
-                                                   uint32_t n_seqs, uint32_t max_batch, hale_decoder** out) {
+// kv: the caller's paged 8-bit cache in place of f32 caches of the decoder's
+// own, or NULL.
+static hale_status decoder_create(hale_ctx* ctx, const hale_decoder_desc* ds, const hale_decoder_layer* lys,
+                                  hale_pool* pool, uint32_t max_len, uint32_t n_seqs, uint32_t max_batch,
+                                  const hale_kv8* kv, hale_decoder** out) {
     if (!ctx || !ds || !lys || !out) return fail(ctx, HALE_E_INVALID_ARGUMENT, "hale_decoder_create: NULL argument");
     *out = nullptr;
     if (n_seqs == 0 || max_batch == 0 || max_batch > 4096)
@@ -2474,8 +2480,24 @@ extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_dec
                     "decoder: bad shape (hidden %u, layers %u, heads %u/%u, head_dim %u, vocab %u, max_len %u)", H,
                     ds->n_layers, nh, nkv, hd, ds->vocab, max_len);
     if (!ds->final_norm) return fail(ctx, HALE_E_INVALID_ARGUMENT, "decoder: final_norm is NULL");
+    if (kv) {
+        if (kv->n_layers != ds->n_layers || kv->n_kv_heads != nkv || kv->head_dim != hd)
+            return fail(ctx, HALE_E_INVALID_ARGUMENT,
+                        "decoder: the cache holds %u layers of %u kv heads of %u, the model has %u of %u of %u",
+                        kv->n_layers, kv->n_kv_heads, kv->head_dim, ds->n_layers, nkv, hd);
+        if ((uint64_t)kv->max_pages * kv->page_tokens < max_len)
+            return fail(ctx, HALE_E_INVALID_ARGUMENT, "decoder: %u positions, a sequence of the cache has room for %llu",
+                        max_len, (unsigned long long)kv->max_pages * kv->page_tokens);
+        // everything else about the cache is checked by its own calls: an empty one here
+        hale_status rk = hale_kv8_resize(ctx, kv, nullptr, nullptr, 0, nullptr);
+        if (rk) return rk;
+    }
     CUDA_TRY(ctx, cudaSetDevice(ctx->device));
     hale_decoder* d = new hale_decoder();
+    if (kv) {
+        d->paged = true;
+        d->kv = *kv;
+    }
     d->ctx = ctx;
     d->device = ctx->device;
     ctx->decoders.insert(d);
@@ -2574,8 +2596,10 @@ extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_dec
     // KV cache: [layer][sequence][position][kv heads * head_dim] f32
     d->seq_stride = (size_t)max_len * kvd;
     const size_t cache = (size_t)d->L * n_seqs * d->seq_stride * 4;
-    if ((r = dec_alloc(ctx, d, cache, reinterpret_cast<void**>(&d->kcache)))) return bail(r);
-    if ((r = dec_alloc(ctx, d, cache, reinterpret_cast<void**>(&d->vcache)))) return bail(r);
+    if (!kv) {
+        if ((r = dec_alloc(ctx, d, cache, reinterpret_cast<void**>(&d->kcache)))) return bail(r);
+        if ((r = dec_alloc(ctx, d, cache, reinterpret_cast<void**>(&d->vcache)))) return bail(r);
+    }
     // attention keeps q and up to 8192 scores in shared memory (below 48 KB);
     // longer contexts keep scores in a [rows][heads][max_len] scratch
     d->smem_scores = std::min<uint32_t>(max_len, 8192u);
@@ -2588,7 +2612,7 @@ extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_dec
     // GQA-grouped attention: one CTA per head at one row (most CTAs for a
     // single token), the whole group (up to 8 heads) in batched steps (each
     // K/V element read once per group)
-    d->gqa = hd <= 256 && hd % 4 == 0;
+    d->gqa = hd <= 256 && hd % 4 == 0 && !kv;
     uint32_t min_cap = d->smem_scores;
     if (d->gqa) {
         const uint32_t G = nh / nkv;
@@ -2621,7 +2645,7 @@ extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_dec
     }
     // one-row steps: attention spread over the GPU when the group fits its
     // shared-memory plan (up to 32 query heads per kv head, head_dim % 8 == 0)
-    if (nh % nkv == 0 && nh / nkv <= 32 && hd % kSplitD == 0 &&
+    if (!kv && nh % nkv == 0 && nh / nkv <= 32 && hd % kSplitD == 0 &&
         (size_t)split_plan((int)(nh / nkv), (int)hd).total * 4 <= kMaxDynSmem) {
         const int G = (int)(nh / nkv);
         d->split_smem = (size_t)split_plan(G, (int)hd).total * 4;
@@ -2642,7 +2666,7 @@ extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_dec
             cudaGetLastError();
         }
     }
-    const size_t score_floats = max_len > min_cap ? B * nh * max_len : 4;
+    const size_t score_floats = max_len > min_cap && !kv ? B * nh * max_len : 4;
     struct { float** p; size_t n; } bufs[] = {{&d->x, B * H}, {&d->x2, B * H}, {&d->moe_out, B * H},
                                                {&d->normed, B * H}, {&d->delta, B * H},
                                                {&d->qkv, B * qkv_rows}, {&d->attn, B * nh * hd},
@@ -2650,14 +2674,27 @@ extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_dec
                                                {&d->h, B * max_inter}, {&d->scores, score_floats}};
     for (auto& b : bufs)
         if ((r = dec_alloc(ctx, d, b.n * 4, reinterpret_cast<void**>(b.p)))) return bail(r);
-    if ((r = dec_alloc(ctx, d, B * 12, reinterpret_cast<void**>(&d->d_rows)))) return bail(r);
+    if ((r = dec_alloc(ctx, d, B * 20, reinterpret_cast<void**>(&d->d_rows)))) return bail(r);
     if (H > 12000) return bail(fail(ctx, HALE_E_INVALID_ARGUMENT, "decoder: hidden %u above 12000", H));
-    if (cudaHostAlloc(reinterpret_cast<void**>(&d->h_rows), B * 12, cudaHostAllocDefault) != cudaSuccess ||
+    if (cudaHostAlloc(reinterpret_cast<void**>(&d->h_rows), B * 20, cudaHostAllocDefault) != cudaSuccess ||
         cudaEventCreateWithFlags(&d->ev_copied, cudaEventDisableTiming) != cudaSuccess ||
         cudaStreamCreateWithFlags(&d->cap, cudaStreamNonBlocking) != cudaSuccess)
         return bail(fail(ctx, HALE_E_CUDA, "decoder: cannot create its step resources"));
     *out = d;
     return HALE_OK;
+}
+
+extern "C" hale_status hale_decoder_create_batched(hale_ctx* ctx, const hale_decoder_desc* ds,
+                                                   const hale_decoder_layer* lys, hale_pool* pool, uint32_t max_len,
+                                                   uint32_t n_seqs, uint32_t max_batch, hale_decoder** out) {
+    return decoder_create(ctx, ds, lys, pool, max_len, n_seqs, max_batch, nullptr, out);
+}
+
+extern "C" hale_status hale_decoder_create_kv8(hale_ctx* ctx, const hale_decoder_desc* ds, const hale_decoder_layer* lys,
+                                               hale_pool* pool, uint32_t max_len, uint32_t max_batch, const hale_kv8* kv,
+                                               hale_decoder** out) {
+    if (!ctx || !kv) return fail(ctx, HALE_E_INVALID_ARGUMENT, "hale_decoder_create_kv8: NULL argument");
+    return decoder_create(ctx, ds, lys, pool, max_len, kv->n_seqs, max_batch, kv, out);
 }
 
 // L2 prefetch descriptor of up to two device ranges (a range that is not
@@ -2677,7 +2714,11 @@ static constexpr uint32_t kNormPrefetchCtas = 32;
 static hale_status decoder_enqueue(hale_ctx* ctx, hale_decoder* d, uint32_t n, float* logits, bool last_logits,
                                    float* hidden, cudaStream_t st) {
     void* stream = st;
-    CUDA_TRY(ctx, cudaMemcpyAsync(d->d_rows, d->h_rows, (size_t)n * 12, cudaMemcpyHostToDevice, st));
+    CUDA_TRY(ctx, cudaMemcpyAsync(d->d_rows, d->h_rows, d->paged ? (size_t)d->max_batch * 20 : (size_t)n * 12,
+                                  cudaMemcpyHostToDevice, st));
+    // a paged decoder's rows once more, positions and sequences apart
+    const int32_t* kv_pos = reinterpret_cast<const int32_t*>(d->d_rows + 3 * (size_t)d->max_batch);
+    const int32_t* kv_seq = kv_pos + d->max_batch;
     hale_status r;
     const int H = (int)d->H, hb = (H + 255) / 256;
     const size_t lstride = (size_t)d->n_seqs * d->seq_stride;
@@ -2701,8 +2742,8 @@ static hale_status decoder_enqueue(hale_ctx* ctx, hale_decoder* d, uint32_t n, f
     float* dspare = d->moe_out;
     for (uint32_t l = 0; l < d->L; l++) {
         const auto& ly = d->layers[l];
-        float* kc = d->kcache + (size_t)l * lstride;
-        float* vc = d->vcache + (size_t)l * lstride;
+        float* kc = d->paged ? nullptr : d->kcache + (size_t)l * lstride;
+        float* vc = d->paged ? nullptr : d->vcache + (size_t)l * lstride;
         // the previous layer's FFN residual folds into this norm; one row: the
         // norm runs inside the q/k/v matvec
         bool fused = false;
@@ -2732,7 +2773,14 @@ static hale_status decoder_enqueue(hale_ctx* ctx, hale_decoder* d, uint32_t n, f
             }
             if ((r = check_launch(ctx, "qk_rope"))) return r;
         }
-        {
+        if (d->paged) {
+            const uint64_t width = (uint64_t)(d->nh + 2 * d->nkv) * d->hd;
+            const float *k = d->qkv + (size_t)d->nh * d->hd, *v = k + (size_t)d->nkv * d->hd;
+            if ((r = hale_kv8_append(ctx, &d->kv, l, k, v, HALE_F32, width, width, kv_seq, kv_pos, n, stream))) return r;
+            if ((r = hale_kv8_attention(ctx, &d->kv, l, d->qkv, HALE_F32, width, kv_seq, kv_pos, n, d->nh, d->scale, 0,
+                                        d->kv_run, d->attn, (uint64_t)d->nh * d->hd, nullptr, stream)))
+                return r;
+        } else {
             ProfScope ps_(ctx, "attention", st);
             if (n == 1 && d->split) {
                 SplitArgs sa{};
@@ -2786,7 +2834,7 @@ static hale_status decoder_enqueue(hale_ctx* ctx, hale_decoder* d, uint32_t n, f
                     d->scores, d->attn, (int)d->smem_scores, d->seq_stride, attn_v_rows((int)d->hd));
             }
         }
-        if ((r = check_launch(ctx, "attn_decode"))) return r;
+        if (!d->paged && (r = check_launch(ctx, "attn_decode"))) return r;
         if ((r = hale_matrix_matvec(ctx, ly.o, d->attn, n, dl, nullptr, stream))) return r;
         hale_moe_layer m{};
         if (ly.is_moe) {
@@ -2869,6 +2917,11 @@ extern "C" hale_status hale_decoder_forward(hale_ctx* ctx, hale_decoder* d, uint
     d->h_rows[0] = token;
     d->h_rows[1] = position;
     d->h_rows[2] = 0;
+    if (d->paged) {
+        d->h_rows[3 * d->max_batch] = position;
+        d->h_rows[4 * d->max_batch] = 0;
+        d->kv_run = 1;
+    }
     const bool capturing = stream_capturing(stream);
     d->copied_recorded = !capturing;
     // per-kernel profiling (hale_ctx_profile) times eager launches only
@@ -2960,6 +3013,17 @@ extern "C" hale_status hale_decoder_step(hale_ctx* ctx, hale_decoder* d, const u
         d->h_rows[3 * i] = tokens[i];
         d->h_rows[3 * i + 1] = positions[i];
         d->h_rows[3 * i + 2] = seqs ? seqs[i] : 0;
+    }
+    if (d->paged) {
+        uint32_t run = 0;
+        d->kv_run = 1;
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t sq = d->h_rows[3 * i + 2];
+            run = i && sq == d->h_rows[3 * i - 1] ? run + 1 : 1;
+            d->kv_run = std::max(d->kv_run, run);
+            d->h_rows[3 * d->max_batch + i] = positions[i];
+            d->h_rows[4 * d->max_batch + i] = sq;
+        }
     }
     hale_status r = decoder_enqueue(ctx, d, n, logits, last_logits_only != 0, hidden, st);
     if (!r) {

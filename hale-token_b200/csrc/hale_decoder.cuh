@@ -113,7 +113,7 @@ __global__ void rmsnorm_kernel(float* __restrict__ x, const float* __restrict__ 
 // RMSNorm of q/k heads, x = x * (scale * w) (norm.rs:30-37, attention.rs:49-56),
 // when the model has it; RoPE (rope.rs:15-43) a' = a c - b s, b' = b c + a s on
 // the pairs (i, i + hd/2); k and v rows appended to the row's sequence cache
-// at its position. qkv: per row [nh*hd | nkv*hd | nkv*hd] as the fused
+// at its position (kcache NULL: they stay in qkv). qkv: per row [nh*hd | nkv*hd | nkv*hd] as the fused
 // projection wrote it. Grid: (nh + 2 nkv, n).
 __global__ void qk_rope_kernel(float* __restrict__ qkv, int nh, int nkv, int hd, const float* __restrict__ q_norm,
                                const float* __restrict__ k_norm, float eps, const float* __restrict__ rope_cos,
@@ -125,9 +125,12 @@ __global__ void qk_rope_kernel(float* __restrict__ qkv, int nh, int nkv, int hd,
     const int kvd = nkv * hd;
     if (head >= nh + 2 * nkv) return;
     qkv += (size_t)r * (nh + 2 * nkv) * hd;
-    kcache += seq * seq_stride;
-    vcache += seq * seq_stride;
+    if (kcache) {
+        kcache += seq * seq_stride;
+        vcache += seq * seq_stride;
+    }
     if (head >= nh + nkv) {  // v head: straight into the cache
+        if (!kcache) return;
         const int vh = head - nh - nkv;
         const float* v = qkv + (size_t)(nh + nkv) * hd + (size_t)vh * hd;
         for (int i = lane; i < hd; i += 32) vcache[(size_t)pos * kvd + vh * hd + i] = v[i];
@@ -160,7 +163,7 @@ __global__ void qk_rope_kernel(float* __restrict__ qkv, int nh, int nkv, int hd,
         x[half + i] = fadd(fmul(b, c[i]), fmul(a, s[i]));
     }
     __syncwarp();
-    if (is_k) {
+    if (is_k && kcache) {
         const int kh = head - nh;
         for (int i = lane; i < hd; i += 32) kcache[(size_t)pos * kvd + kh * hd + i] = x[i];
     }

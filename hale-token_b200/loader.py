@@ -540,7 +540,7 @@ def cache_policy(config, record_bytes, budget_bytes, routing_counts=None):
 
 
 def load_decoder(ctx, directory, expert_dtype=None, max_len=None, policy=None, expert_hbm_bytes=None,
-                 routing_counts=None, n_seqs=1, max_batch=1):
+                 routing_counts=None, n_seqs=1, max_batch=1, kv8=None):
     """Builds (decoder, pool, config) from a model directory: a Hugging Face
     checkpoint (config.json + safetensors) or a converted one (config.json,
     dense.safetensors, experts.hpk). Dense weights as stored; experts into an
@@ -549,7 +549,8 @@ def load_decoder(ctx, directory, expert_dtype=None, max_len=None, policy=None, e
     experts of `routing_counts` -- a RoutingStats, or [MoE layers, experts]
     counts -- pinned first) is given. max_len: KV-cache
     positions (default the config's max_position_embeddings); n_seqs /
-    max_batch: KV caches and rows per Decoder.step."""
+    max_batch: KV caches and rows per Decoder.step; kv8: a Kv8 that holds the
+    keys and values in place of f32 caches."""
     w = ModelWeights(directory, expert_dtype)
     cfg = w.config
     if isinstance(routing_counts, RoutingStats):
@@ -564,5 +565,5 @@ def load_decoder(ctx, directory, expert_dtype=None, max_len=None, policy=None, e
             for e in range(cfg.num_experts):
                 pool.upload(j, e, w.expert_record(j, e))
     dec = hale.Decoder(ctx, w.dims, w.layers, w.embed, w.lm_head, w.final_norm, pool,
-                       max_len or cfg.max_position_embeddings, n_seqs, max_batch)
+                       max_len or cfg.max_position_embeddings, n_seqs, max_batch, kv8)
     return dec, pool, cfg

@@ -623,6 +623,18 @@ HALE_API hale_status hale_kv8_compact(hale_ctx* ctx, const hale_kv8* kv, int32_t
 HALE_API hale_status hale_kv8_copy(hale_ctx* ctx, const hale_kv8* kv, const int32_t* src, const int32_t* dst, uint32_t n,
                                    void* stream);
 
+/* A decoder whose keys and values live in the caller's cache instead of f32
+ * caches of its own (hale_decoder_create_batched otherwise; n_seqs is the
+ * cache's). Every step appends its rows to the cache and attends over it, so
+ * logits are those of the f32 cache but for the codes' rounding. The buffers
+ * kv names must outlive the decoder, and the tokens of a step must have their
+ * pages (hale_kv8_resize before the step; a missing page is reported as
+ * HALE_E_DEVICE_CHECK). head_dim a multiple of 16 up to 256; max_len at most
+ * what a sequence of the cache can have. */
+HALE_API hale_status hale_decoder_create_kv8(hale_ctx* ctx, const hale_decoder_desc* desc,
+                                             const hale_decoder_layer* layers, hale_pool* experts, uint32_t max_len,
+                                             uint32_t max_batch, const hale_kv8* kv, hale_decoder** out);
+
 /* ---- drafted tokens ----------------------------------------------------------
  * Speculative sampling's check, the counterpart of Sampler::sample
  * (src/generate/sampler.rs:80-123) for several drafted tokens at once; the

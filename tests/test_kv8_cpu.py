@@ -60,5 +60,7 @@ def test_null_handles_are_refused():
     assert lib.hale_kv8_compact(None, kv, None, None, None) == bad
     assert lib.hale_kv8_copy(None, kv, None, None, 1, None) == bad
     assert lib.hale_verify_drafts(None, None, 0, 0, None, None, 0, None, 1, 1, 1, 1.0, None, None, None, None, None) == bad
+    out = C.c_void_p()
+    assert lib.hale_decoder_create_kv8(None, None, None, None, 1, 1, kv, C.byref(out)) == bad
     buf = C.create_string_buffer(128)
-    assert lib.hale_last_error(None, buf, 128) == bad and b"ctx is NULL" in buf.value
+    assert lib.hale_last_error(None, buf, 128) == bad and b"NULL" in buf.value

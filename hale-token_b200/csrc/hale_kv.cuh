@@ -229,23 +229,51 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvArgs c, KvAppend a) {
         const float s = fmaxf(old, kv_want(amax));
         const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
         const bool grown = old > 0.0f && s > old;
+        // x inv + 1.5 2^23 has the rounded quotient in its low byte; where the
+        // remainder is half a code or more (a tie, a quotient rounded across
+        // one, or no number) the lane's warp takes the careful path instead
+        bool check = false;
+        const float half = 0.5f * s;
 #pragma unroll
         for (int j = 0; j < kKvBlock; j++) {
-            const bool held = s_slot[b][j] < 0;
-            if (held && !grown) continue;
+            if (s_slot[b][j] < 0) continue;
 #pragma unroll
             for (int u = 0; u < NV; u++) {
-                const int d = 4 * (lane + 32 * u);
-                if (d >= c.hd) continue;
-                uint32_t* at = reinterpret_cast<uint32_t*>(codes + (size_t)j * c.hd + d);
-                uint32_t w = 0;
-                const uint32_t was = held ? *at : 0u;
+                uint32_t t[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int q = held ? kv_recode((int8_t)(was >> (8 * e)), old, s) : kv_code(x[j][u][e], s, inv);
-                    w |= (uint32_t)(q & 0xff) << (8 * e);
+                    const float y = __fmaf_rn(x[j][u][e], inv, 12582912.0f);
+                    check |= !(fabsf(__fmaf_rn(-(y - 12582912.0f), s, x[j][u][e])) < half);
+                    t[e] = __float_as_uint(y);
                 }
-                *at = w;
+                const int d = 4 * (lane + 32 * u);
+                if (d < c.hd)
+                    *reinterpret_cast<uint32_t*>(codes + (size_t)j * c.hd + d) =
+                        __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+            }
+        }
+        // the careful path, and codes that were there before; seldom, so kept
+        // short (each pass of a kernel fetches its code anew)
+        const bool again = __any_sync(0xffffffffu, check);
+        if (again || grown) {
+#pragma unroll 1
+            for (int j = 0; j < kKvBlock; j++) {
+                const int row = s_slot[b][j];
+                if (row >= 0 ? !again : !grown) continue;
+#pragma unroll 1
+                for (int d = 4 * lane; d < c.hd; d += 128) {
+                    uint32_t* at = reinterpret_cast<uint32_t*>(codes + (size_t)j * c.hd + d);
+                    const uint32_t was = *at;
+                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (row >= 0) load4<DT>(src, (size_t)row * stride + (size_t)head * c.hd + d, y);
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int q = row >= 0 ? kv_code(y[e], s, inv) : kv_recode((int8_t)(was >> (8 * e)), old, s);
+                        w |= (uint32_t)(q & 0xff) << (8 * e);
+                    }
+                    *at = w;
+                }
             }
         }
         __syncwarp();

@@ -843,14 +843,16 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 && NT == 1 ? 3 : 2) kv_
 // many columns: 64 of them per tile, codes widened to f16 once for all
 //
 // Four warps of 16 columns each. A unit of UT tokens arrives as codes by
-// asynchronous copies (one unit ahead), is widened to f16 tiles in shared
+// asynchronous copies (during the unit before it), is widened to f16 tiles in shared
 // memory by all warps, and feeds both products from there: S = q K^T with q
 // from shared memory, O += P V with P straight from S's registers. q is scaled
 // by a power of two to at most 2^14: exact in f16 for f16 and (down to 2^-38
 // of the row's largest value) bf16, two f16 (22 bits) for f32. Tiles lie in
 // rows of 2 DP bytes whose 16-byte pieces are xor-ed with the row's number, so
-// that neither the stores nor the matrix loads meet a bank twice.
-// Bound by the matrix instructions (m16n8k16 issues once in 8 cycles).
+// that the matrix loads meet no bank twice.
+// Bound by instruction issue beside the matrix instructions (one m16n8k16 in 8
+// cycles): a warp's unit of 64 tokens is 128 of them and about 1000 others,
+// half of those the softmax.
 // ---------------------------------------------------------------------------
 constexpr int kManyWarps = 4, kManyThreads = 32 * kManyWarps, kManyCols = 16 * kManyWarps, kManyCost = 2;
 
@@ -861,8 +863,8 @@ struct ManyCfg {
     static constexpr int CODES = UT * DP;                 // bytes of a unit's keys (or values)
     static constexpr int QUERY = kManyCols * DP * 2;      // one f16 part of the queries
     static constexpr int TILE = UT * DP * 2;              // f16 keys (or values)
-    static constexpr int SMEM = SPLIT * QUERY + 2 * TILE + 4 * CODES;
-    static constexpr int PER_SM = DP == 256 && SPLIT == 2 ? 1 : 2;
+    static constexpr int SMEM = SPLIT * QUERY + 2 * TILE + 2 * CODES;
+    static constexpr int PER_SM = SPLIT == 1 && DP <= 128 ? 3 : 2;
 };
 
 __device__ __forceinline__ void load_matrix(uint32_t (&r)[4], uint32_t addr) {
@@ -957,7 +959,7 @@ __global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn
                     pages_next = find(u + HELD);
                 }
                 const int stage = (u - u0) & 1;
-                const uint32_t dst = s_codes + stage * 2 * Cfg::CODES + 16 * tid;
+                const uint32_t dst = s_codes + 16 * tid;
 #pragma unroll
                 for (int r = 0; r < UT; r += STEP) {
                     // a warp's rows lie in one block
@@ -1061,21 +1063,21 @@ __global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn
             const int t0 = u * UT, stage = (u - u0) & 1;
             cp_async_wait<0>();
             __syncthreads();  // the codes are there, and no one reads the tiles any more
-            fetch(u + 1);
 #pragma unroll
             for (int r = 0; r < UT; r += STEP) {
-                const int t = r + my_row, odd = my_piece >> 2 & 1;
+                const int t = r + my_row;
 #pragma unroll
                 for (int v = 0; v < 2; v++) {
-                    const uint4 x = load_shared16(s_codes + (2 * stage + v) * Cfg::CODES + 16 * tid + r * DP);
+                    const uint4 x = load_shared16(s_codes + v * Cfg::CODES + 16 * tid + r * DP);
                     const uint2 h0 = codes_f16(x.x), h1 = codes_f16(x.y), h2 = codes_f16(x.z), h3 = codes_f16(x.w);
                     const uint4 lo = make_uint4(h0.x, h0.y, h1.x, h1.y), hi = make_uint4(h2.x, h2.y, h3.x, h3.y);
                     const uint32_t to = (v ? s_v : s_k) + t * ROW;
-                    store_shared16(to + 16 * ((2 * my_piece + odd) ^ (t & 7)), odd ? hi : lo);
-                    store_shared16(to + 16 * ((2 * my_piece + 1 - odd) ^ (t & 7)), odd ? lo : hi);
+                    store_shared16(to + 16 * ((2 * my_piece) ^ (t & 7)), lo);
+                    store_shared16(to + 16 * ((2 * my_piece + 1) ^ (t & 7)), hi);
                 }
             }
             __syncthreads();
+            fetch(u + 1);
             if (t0 >= any_hi || t0 + UT <= seg.lo) continue;  // nothing of it for this warp's columns
 
             // ---- S = q K^T ----
@@ -1116,16 +1118,13 @@ __global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn
                 vs[b] = none_of_it ? 0.0f : block.vs;
                 whole = whole && !none_of_it;
             }
-            unsigned hidden[2] = {0, 0};  // bit 2 i + e & 1 of token 8 i + 2 q4 + (e & 1)
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < UT / 8; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int t = t0 + 8 * i + 2 * q4 + (e & 1);
-                        if (page[i / 2] < 0 || t >= end[e >> 1] || t < begin[e >> 1]) hidden[e >> 1] |= 1u << (2 * i + (e & 1));
-                    }
-            }
+            // softmax and second product; WHOLE: every column sees every token
+            auto weigh = [&](auto whole_) {
+            constexpr bool WHOLE = decltype(whole_)::value;
+            auto hidden = [&](int i, int e) {  // token 8 i + 2 q4 + (e & 1)
+                const int t = t0 + 8 * i + 2 * q4 + (e & 1);
+                return !WHOLE && (page[i / 2] < 0 || t >= end[e >> 1] || t < begin[e >> 1]);
+            };
             float top[2] = {m[0], m[1]}, vmax = vtop;
 #pragma unroll
             for (int b = 0; b < NB; b++) vmax = fmaxf(vmax, vs[b]);
@@ -1134,7 +1133,7 @@ __global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float y = s[i][e] * (ks[i / 2] * qs[e >> 1]);
-                    top[e >> 1] = fmaxf(top[e >> 1], hidden[e >> 1] >> (2 * i + (e & 1)) & 1u ? none : y);
+                    top[e >> 1] = fmaxf(top[e >> 1], hidden(i, e) ? none : y);
                 }
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || vmax > vtop)) {
                 const float fix_v = vmax > 0.0f ? vtop / vmax : 1.0f;
@@ -1168,7 +1167,7 @@ __global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn
                     for (int e = 0; e < 4; e++) {
                         const int i = 2 * b + j;
                         float x = exp2_fast(fmaf(s[i][e], ks[b] * qs[e >> 1], -base[e >> 1]));
-                        if (hidden[e >> 1] >> (2 * i + (e & 1)) & 1u) x = 0.0f;
+                        if (hidden(i, e)) x = 0.0f;
                         l[e >> 1] += x;
                         w[e] = x * fv;
                     }
@@ -1193,6 +1192,9 @@ __global__ void __launch_bounds__(kManyThreads, ManyCfg<DT, DP>::PER_SM) kv_attn
                     }
                 }
             }
+            };
+            if (whole) weigh(std::true_type{});
+            else weigh(std::false_type{});
         }
         cp_async_wait<0>();
 

@@ -268,6 +268,8 @@ extern "C" hale_status hale_kv8_append(hale_ctx* ctx, const hale_kv8* kv, uint32
         (r = check_rows(ctx, what, "k", k, dtype, k_stride, width)) ||
         (r = check_rows(ctx, what, "v", v, dtype, v_stride, width)))
         return r;
+    // every CTA looks over the whole list: 2^18 rows are some milliseconds
+    if (n > (1u << 18)) return fail(ctx, HALE_E_INVALID_ARGUMENT, "%s: %u rows (up to 2^18)", what, n);
     OnDevice on(ctx);
     CUDA_TRY(ctx, on.err);
     const KvArgs c = layer_args(ctx, kv, layer);
@@ -338,6 +340,9 @@ extern "C" hale_status hale_kv8_attention(hale_ctx* ctx, const hale_kv8* kv, uin
     OnDevice on(ctx);
     CUDA_TRY(ctx, on.err);
     const KvArgs c = layer_args(ctx, kv, layer);
+    // a row's units are counted in 32 bits (no tile has fewer than 32 tokens a unit)
+    if ((uint64_t)kv->n_kv_heads * (n_heads / kv->n_kv_heads / 8 + 1) * ((uint64_t)c.capacity() / 32 + 8) > 0x7fffffffull)
+        return fail(ctx, HALE_E_UNSUPPORTED, "%s: sequences of %u pages over %u heads are too long", what, kv->max_pages, n_heads);
     KvAttn a{};
     a.q = q;
     a.out = out;

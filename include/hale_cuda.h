@@ -563,7 +563,7 @@ typedef struct {
  * `stride` elements apart, 16-byte aligned) into layer `layer`: row r is token
  * positions[r] of sequence seqs[r] (device arrays; seqs NULL: sequence 0). A
  * row with a negative sequence or position is left out; of two rows for one
- * token the later counts. The rows of one call that fall into one block of 16
+ * token the later counts. Up to 2^18 rows. The rows of one call that fall into one block of 16
  * tokens are taken together: scale = max |x| / 127 (at least 2^-100), or the
  * block's scale so far if that is larger; codes already in the block are
  * rounded again when the scale grows, and a row for the block's first token

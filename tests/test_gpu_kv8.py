@@ -221,6 +221,28 @@ def test_scales_far_apart_and_zero(ctx, dtype, run):
     check_attention(out, lse, attention64(kv, 0, qt.double().cpu().numpy(), [0] * 6, pos, 0.25, 0), dtype)
 
 
+@pytest.mark.parametrize("run", [1, 16])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_a_query_that_is_no_number_spoils_its_own_head_alone(ctx, dtype, run):
+    kv = filled(ctx, 9, [300], 2, 64, 32)
+    g = np.random.default_rng(4)
+    q = torch.from_numpy(g.normal(0, 1, (3, 4, 64)).astype(np.float32)).cuda().to(DT[dtype])
+    q[1, 2, 7] = float("nan")
+    q[2, 0, 5] = float("inf")
+    out, lse = torch.zeros_like(q), torch.zeros((3, 4), device="cuda")
+    kv.attention(0, q, out, ints([299, 120, 7]), ints([0, 0, 0]), run=run, lse=lse)
+    ctx.check()
+    bad = torch.zeros((3, 4), dtype=torch.bool)
+    bad[1, 2] = bad[2, 0] = True
+    assert torch.equal(out.float().isnan().all(-1).cpu(), bad) and torch.equal(out.float().isnan().any(-1).cpu(), bad)
+    assert torch.equal(lse.isnan().cpu(), bad)
+    clean = torch.where(bad[..., None].cuda(), torch.zeros_like(q), q)
+    want = attention64(kv, 0, clean.double().cpu().numpy(), [0] * 3, [299, 120, 7], np.float64(np.float32(64 ** -0.5)), 0)
+    keep = (~bad).numpy()
+    o, z, worst, top = want
+    check_attention(out.cpu()[torch.from_numpy(keep)], lse.cpu()[torch.from_numpy(keep)], (o[keep], z[keep], worst[keep], top[keep]), dtype)
+
+
 def test_rows_apart_other_layers_and_other_streams(ctx):
     """q and out as slices of wider rows, a middle layer, a side stream, and
     the same call twice: the same bits."""
